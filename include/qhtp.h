@@ -332,6 +332,94 @@ QhtpStatus qhtp_gdn_solve_u16(const uint16_t *A, int64_t n_chunks, int32_t C, in
                               int32_t zpT, float sT, uint16_t *T, void *stream);
 
 /* ------------------------------------------------------------------------------------------
+ * 8-bit paged KV cache: writing K and V rows, reading them back, attention over the cache.
+ * No counterpart in the reference, whose attention stays with the QNN runtime.
+ *
+ * The cache holds int8 codes [num_blocks, kv_heads, block_size, head_dim] for K and for V, and one
+ * float32 scale per (block, kv head) of each, [num_blocks, kv_heads]: value = code * scale.  Token p of
+ * sequence b is slot p % block_size of block block_table[b][p / block_size].  block_size is 16, 32, 64 or
+ * 128, head_dim 64, 128 or 256.  A table entry outside [0, num_blocks) maps nothing: rows written there
+ * are dropped, and what is read there, or attended to, is NaN.  Nothing outside the cache is touched.
+ *
+ * Writing to tile (block, kv head), float32 arithmetic: s_new = max|x| / 127 over the new rows x in it (0
+ * below 2^-64).  If slot 0 is among them the tile starts anew with scale s = s_new, else s = max(old scale,
+ * s_new) and, where s grew, the old codes become rint(code * (old / s)).  New codes are
+ * clamp(rint(x * (1 / s)), -127, 127).  A NaN or an infinity among the rows, or in the old scale, makes the
+ * tile's scale NaN until it starts anew.  Each block that is written belongs to one sequence of the call,
+ * and a sequence's tokens are written in order: a later write may start anywhere at or below the end, and
+ * then what lay beyond its last row is lost.
+ * ------------------------------------------------------------------------------------------ */
+typedef enum QhtpDtype { QHTP_DTYPE_BF16 = 0, QHTP_DTYPE_F16 = 1, QHTP_DTYPE_F32 = 2 } QhtpDtype;
+
+typedef struct QhtpKv8Cache {
+  int8_t *k, *v;              /* 16-byte aligned */
+  float *k_scale, *v_scale;
+  int64_t num_blocks;
+  uint32_t kv_heads, head_dim, block_size, reserved; /* reserved: 0 */
+} QhtpKv8Cache;
+
+/* The sequences of a call.  seq_start NULL: each has `tokens` rows, and row (b, t) lies at
+ * b * batch_stride + t * token_stride.  seq_start int32 [batch + 1]: sequence b has the rows seq_start[b] to
+ * seq_start[b + 1] of `total`, row i lies at i * token_stride, and `tokens` is at least the largest count (rows of a
+ * sequence beyond that many may be left out).  Starts outside [0, total] or falling give no rows. */
+typedef struct QhtpKv8Seqs {
+  const int32_t *block_table; /* [batch, max_blocks], rows table_stride apart */
+  const int32_t *seq_start;
+  int64_t table_stride, total;
+  uint32_t max_blocks, batch, tokens, reserved;
+} QhtpKv8Seqs;
+
+/* Rows of heads.  Strides in elements; head_dim is contiguous; the base and every stride in bytes are
+ * multiples of 16. */
+typedef struct QhtpKv8Rows {
+  void *data;
+  int64_t batch_stride, token_stride, head_stride;
+} QhtpKv8Rows;
+
+typedef struct QhtpKv8Move {
+  QhtpKv8Cache cache;
+  QhtpKv8Seqs seqs;
+  const int32_t *first;       /* [batch] cache position of each sequence's first row */
+  QhtpKv8Rows k, v;
+  uint32_t dtype, reserved;   /* QhtpDtype of the rows */
+  void *stream;
+} QhtpKv8Move;
+
+/* Quantize the rows k, v [.., kv_heads, head_dim] into the cache at positions first[b], first[b] + 1, ...
+ * (a negative first counts as 0).  Asynchronous. */
+QhtpStatus qhtp_kv8_write(const QhtpKv8Move *move);
+
+/* The cache's rows at positions first[b], ... as k, v: code * scale in float32, rounded once to dtype.  A position
+ * below 0 or past the block table reads as NaN.  Asynchronous. */
+QhtpStatus qhtp_kv8_read(const QhtpKv8Move *move);
+
+/* Attention: out = softmax(scale * q K^T) V per head, query head h on kv head h / (q_heads / kv_heads), over
+ * the first lengths[b] tokens of sequence b, of which the T query tokens are the last: query token t stands at
+ * position p = lengths[b] - T + t, and with `causal` sees the keys 0..p, with `window` > 0 (causal only) the
+ * keys p - window + 1..p, else all of them.  A row that sees no key gives zeros.  A negative length counts as 0, one
+ * past the block table as its end.  Scores, maxima, sums and outputs are float32; q is taken to f16 by a power
+ * of two per row (all bits of elements within 2^-29 of the row's largest), probabilities are rounded to f16.
+ * Scales are at least 0; a V scale below 2^-64 counts as 0. */
+typedef struct QhtpKv8Attention {
+  QhtpKv8Cache cache;
+  QhtpKv8Seqs seqs;
+  const int32_t *lengths;     /* [batch] */
+  QhtpKv8Rows q, out;         /* [.., q_heads, head_dim], dtype bf16 or f16 */
+  float *lse;                 /* [rows, q_heads] natural log of the sums of exponentials, -inf for no key; may be NULL */
+  uint32_t dtype, q_heads;
+  uint32_t causal, window;
+  float scale;                /* finite, > 0 */
+  uint32_t max_len;           /* about the largest length: sizes the grid, changes no result */
+  void *workspace;            /* qhtp_kv8_attention_workspace_bytes; 256-byte aligned */
+  size_t workspace_bytes;
+  void *stream;
+} QhtpKv8Attention;
+
+/* Device workspace of the call (0 for many): reads the shapes, dtype, window and max_len of *run only. */
+size_t qhtp_kv8_attention_workspace_bytes(const QhtpKv8Attention *run);
+QhtpStatus qhtp_kv8_attention(const QhtpKv8Attention *run);
+
+/* ------------------------------------------------------------------------------------------
  * Host-only helpers (no GPU needed).
  * ------------------------------------------------------------------------------------------ */
 

@@ -62,6 +62,42 @@ class QhtpPreparedRun(C.Structure):
     ]
 
 
+class QhtpKv8Cache(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("num_blocks", C.c_int64), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("block_size", C.c_uint32),
+        ("reserved", C.c_uint32),
+    ]
+
+
+class QhtpKv8Seqs(C.Structure):
+    _fields_ = [
+        ("block_table", C.c_void_p), ("seq_start", C.c_void_p), ("table_stride", C.c_int64), ("total", C.c_int64),
+        ("max_blocks", C.c_uint32), ("batch", C.c_uint32), ("tokens", C.c_uint32), ("reserved", C.c_uint32),
+    ]
+
+
+class QhtpKv8Rows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("batch_stride", C.c_int64), ("token_stride", C.c_int64),
+                ("head_stride", C.c_int64)]
+
+
+class QhtpKv8Move(C.Structure):
+    _fields_ = [
+        ("cache", QhtpKv8Cache), ("seqs", QhtpKv8Seqs), ("first", C.c_void_p), ("k", QhtpKv8Rows), ("v", QhtpKv8Rows),
+        ("dtype", C.c_uint32), ("reserved", C.c_uint32), ("stream", C.c_void_p),
+    ]
+
+
+class QhtpKv8Attention(C.Structure):
+    _fields_ = [
+        ("cache", QhtpKv8Cache), ("seqs", QhtpKv8Seqs), ("lengths", C.c_void_p), ("q", QhtpKv8Rows),
+        ("out", QhtpKv8Rows), ("lse", C.c_void_p), ("dtype", C.c_uint32), ("q_heads", C.c_uint32),
+        ("causal", C.c_uint32), ("window", C.c_uint32), ("scale", C.c_float), ("max_len", C.c_uint32),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("stream", C.c_void_p),
+    ]
+
+
 # every symbol include/qhtp.h declares: name -> (restype, argtypes)
 SIGNATURES = {
     "qhtp_status_string": (C.c_char_p, [C.c_int]),
@@ -104,6 +140,11 @@ SIGNATURES = {
                                          C.c_int32, C.c_void_p]),
     "qhtp_gdn_solve_u16": (C.c_int, [C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_float, C.c_int32,
                                      C.c_float, C.c_void_p, C.c_void_p]),
+    # the kv8 structures are passed by address, as ctypes structures or packed by struct (see kv8.py)
+    "qhtp_kv8_write": (C.c_int, [C.c_void_p]),
+    "qhtp_kv8_read": (C.c_int, [C.c_void_p]),
+    "qhtp_kv8_attention_workspace_bytes": (C.c_size_t, [C.c_void_p]),
+    "qhtp_kv8_attention": (C.c_int, [C.c_void_p]),
     "qhtp_requant_code_host": (C.c_int32, [C.c_int64, C.c_uint64, C.c_int32, C.c_uint32, C.c_int32, C.c_uint64,
                                            C.c_uint64, C.c_int32, C.c_int32, C.c_int32]),
 }

@@ -1,0 +1,259 @@
+// Pieces shared by the 8-bit KV cache kernels: the paged layout, the sequences of a call, and the
+// int8 -> f16 conversion that feeds the tensor cores.
+//
+// The cache holds int8 codes [num_blocks, kv_heads, block_size, head_dim] for K and for V and one
+// float32 scale per (block, kv head) of each; value = code * scale.  Token p of sequence b is slot
+// p % block_size of block block_table[b, p / block_size].  A (block, kv head) tile is contiguous.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "internal.h"
+#include "ptx.cuh"
+
+namespace qhtp {
+namespace kv8 {
+
+// Scales below this count as zero when a block is written.  The attention kernels divide by V scales
+// (see kv8_decode.cu): from 2^-64 up, 1 / scale summed over 2^31 keys stays far inside float32.
+constexpr float kScaleMin = 5.421010862427522e-20f;  // 2^-64
+
+struct Pages {
+  int8_t* k;
+  int8_t* v;
+  float* k_scale;
+  float* v_scale;
+  long long num_blocks;
+  int heads;      // kv heads
+  int bs_log2;    // block_size = 1 << bs_log2
+};
+
+struct Seqs {
+  const int32_t* table;   // [batch, max_blocks]
+  long long table_stride;
+  int max_blocks;
+  int batch;
+  const int32_t* start;   // [batch + 1] rows of each sequence, or null: `tokens` rows each
+  int tokens;             // rows of each sequence, or (start given) the most of any
+  long long total;        // rows in all (start given)
+};
+
+struct Rows {
+  void* data;
+  long long batch_stride, token_stride, head_stride;  // in elements; head_dim is contiguous
+};
+
+// Rows of sequence b: their number, and the index that token_stride multiplies for the first.  A start
+// that lies outside [0, total] gives no rows.
+__device__ __forceinline__ int seq_rows(const Seqs& s, int b, long long& first) {
+  if (s.start == nullptr) {
+    first = 0;
+    return s.tokens;
+  }
+  const long long a = s.start[b], e = s.start[b + 1];
+  first = a;
+  return a < 0 || e > s.total || e <= a ? 0 : static_cast<int>(e - a);
+}
+
+// Block of a sequence's block index, or -1 where the table has none or names one outside the cache.
+__device__ __forceinline__ long long block_of(const Seqs& s, const Pages& p, int b, long long idx) {
+  if (idx < 0 || idx >= s.max_blocks) return -1;
+  const long long id = s.table[b * s.table_stride + idx];
+  return id >= 0 && id < p.num_blocks ? id : -1;
+}
+
+// Four int8 codes (one word) -> two half2, exactly: code + 128 is put into the low mantissa bits of
+// the half 1024, and 1024 + 128 is taken off.  Three integer / half2 instructions per two codes less
+// a shared xor, against four conversions.
+__device__ __forceinline__ uint32_t sub_1152(uint32_t h) {
+  const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), bias);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ void codes_to_half2(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  w ^= 0x80808080u;
+  lo = sub_1152(prmt(w, 0x64646464u, 0x4140u));
+  hi = sub_1152(prmt(w, 0x64646464u, 0x4342u));
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ float nan_f32() { return __uint_as_float(0x7fffffffu); }
+
+// 16 bytes of T -> float32
+template <typename T>
+struct Vec;
+template <>
+struct Vec<float> {
+  static constexpr int n = 4;
+  __device__ static void load(const uint4& r, float (&f)[4]) {
+    f[0] = __uint_as_float(r.x), f[1] = __uint_as_float(r.y), f[2] = __uint_as_float(r.z), f[3] = __uint_as_float(r.w);
+  }
+  __device__ static uint4 store(const float (&f)[4]) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+};
+template <>
+struct Vec<__half> {
+  static constexpr int n = 8;
+  __device__ static void load(const uint4& r, float (&f)[8]) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = t.x, f[2 * i + 1] = t.y;
+    }
+  }
+  __device__ static uint4 store(const float (&f)[8]) {
+    return make_uint4(pack_half2(f[0], f[1]), pack_half2(f[2], f[3]), pack_half2(f[4], f[5]), pack_half2(f[6], f[7]));
+  }
+};
+template <>
+struct Vec<__nv_bfloat16> {
+  static constexpr int n = 8;
+  __device__ static void load(const uint4& r, float (&f)[8]) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(w[i] << 16), f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+  __device__ static uint32_t pack(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  __device__ static uint4 store(const float (&f)[8]) {
+    return make_uint4(pack(f[0], f[1]), pack(f[2], f[3]), pack(f[4], f[5]), pack(f[6], f[7]));
+  }
+};
+
+}  // namespace kv8
+
+// kv8_cache.cu
+struct Kv8Move {
+  kv8::Pages pages;
+  kv8::Seqs seqs;
+  const int32_t* first;   // cache position of each sequence's first row
+  kv8::Rows k, v;
+  uint32_t dtype;
+  int head_dim;
+  cudaStream_t stream;
+};
+cudaError_t launch_kv8_write(const Kv8Move& m);
+cudaError_t launch_kv8_read(const Kv8Move& m);
+
+// Attention over the cache.  Query row r of a (sequence, kv head) is token r / group, head r % group of
+// the kv head's group; token t of T stands at position length - T + t.
+struct Kv8Attn {
+  kv8::Pages pages;
+  kv8::Seqs seqs;
+  const int32_t* lengths;
+  kv8::Rows q, out;
+  float* lse;             // [rows, q_heads] or null
+  int bf16;               // q and out: bf16, else f16
+  int head_dim, q_heads, group;
+  int causal, window;     // window 0: none
+  float scale_log2;       // softmax scale * log2(e)
+  int max_len;            // the caller's bound on the lengths (sizes the grid only)
+  // a launch's plan: rows per CTA, row groups of a sequence, keys per chunk, chunks
+  int tile_rows, row_groups, chunk, chunks;
+  float* part;            // workspace (chunks > 1): unnormalised rows, then their maxima and sums
+  cudaStream_t stream;
+};
+
+namespace kv8 {
+
+// Keys that rows [r0, r1) of a sequence of T tokens see, over all of the rows.
+struct Span {
+  int lo, hi;
+};
+__device__ __forceinline__ Span row_span(const Kv8Attn& a, int len, int T, int r0, int r1) {
+  Span s{0, len};
+  if (a.causal) s.hi = min(len, len - T + (r1 - 1) / a.group + 1);
+  if (a.window) s.lo = max(0, len - T + r0 / a.group - a.window + 1);
+  return s;
+}
+__device__ __forceinline__ int seq_length(const Kv8Attn& a, int b) {
+  const long long cap = static_cast<long long>(a.seqs.max_blocks) << a.pages.bs_log2;
+  const int len = max(a.lengths[b], 0);
+  return len < cap ? len : static_cast<int>(cap);
+}
+// Chunk c of a span: chunks start at a multiple of 32 keys, and the last takes what is left.
+__device__ __forceinline__ Span chunk_span(const Kv8Attn& a, const Span& s, int c) {
+  const long long lo = (s.lo & ~31) + static_cast<long long>(c) * a.chunk;
+  const long long hi = c == a.chunks - 1 ? s.hi : min(static_cast<long long>(s.hi), lo + a.chunk);
+  return lo < hi ? Span{static_cast<int>(lo), static_cast<int>(hi)} : Span{0, 0};
+}
+// Offset of a (sequence, kv head, row group, chunk) part in rows.
+__device__ __forceinline__ long long part_row(const Kv8Attn& a, int b, int h, int rg, int c) {
+  return (((static_cast<long long>(b) * a.pages.heads + h) * a.row_groups + rg) * a.chunks + c) * a.tile_rows;
+}
+__device__ __forceinline__ long long part_rows(const Kv8Attn& a) {
+  return static_cast<long long>(a.seqs.batch) * a.pages.heads * a.row_groups * a.chunks * a.tile_rows;
+}
+
+// A block's constants for the softmax: with c = scale * log2(e) * k_scale and w = v_scale, a key's
+// exponent is q . code * c + log2(w), and 1 / w takes w out of the row's sum again.  A v_scale below
+// kScaleMin counts as zero: w is kScaleMin then, and inv_w = kZeroTile tells that the codes add nothing.
+struct BlockScales {
+  float c, log2_w, inv_w;
+};
+constexpr float kZeroTile = 36893488147419103232.0f;  // 2^65
+__device__ __forceinline__ BlockScales block_scales(const Kv8Attn& a, long long id, int h) {
+  if (id < 0) return {nan_f32(), nan_f32(), nan_f32()};
+  const long long t = id * a.pages.heads + h;
+  const float w = a.pages.v_scale[t];
+  const float v = w < kScaleMin ? kScaleMin : w;  // a NaN stays
+  return {a.pages.k_scale[t] * a.scale_log2, log2f(v), w < kScaleMin ? kZeroTile : 1.0f / v};
+}
+
+// 2^-e and the factor 2^e that brings a row of largest magnitude `top` to [2^14, 2^15): q then fits f16 without
+// overflow, and every element within 2^-29 of the largest keeps all of its bits.
+__device__ __forceinline__ void row_factor(float top, float& up, float& down) {
+  const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;  // top >= 0
+  if (top == 0.0f || e >= 128) {  // nothing to scale, or not finite
+    up = down = 1.0f;
+    return;
+  }
+  // e >= -126 (a subnormal counts as 2^-127): 14 - e <= 141 can pass 2^127, so it is capped there
+  const int up_e = min(14 - max(e, -127), 126);
+  up = __uint_as_float(static_cast<uint32_t>(up_e + 127) << 23);
+  down = __uint_as_float(static_cast<uint32_t>(127 - up_e) << 23);
+}
+
+// Eight elements of a finished row: out = o / sum, and (with the row's first eight) its lse.  A row that
+// sees no key has sum 0: zeros, and an lse of -infinity.
+__device__ __forceinline__ void write_row8(const Kv8Attn& a, int b, long long row0, int row, int h, int d0,
+                                           const float (&o)[8], float sum, float top) {
+  const int t = row / a.group, head = h * a.group + row - t * a.group;
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = o[e] * inv;
+  uint16_t* to = static_cast<uint16_t*>(a.out.data) + b * a.out.batch_stride + (row0 + t) * a.out.token_stride +
+                 head * a.out.head_stride + d0;
+  *reinterpret_cast<uint4*>(to) = a.bf16 ? Vec<__nv_bfloat16>::store(v) : Vec<__half>::store(v);
+  if (a.lse != nullptr && d0 == 0) {
+    const long long at = (a.seqs.start ? row0 : static_cast<long long>(b) * a.seqs.tokens) + t;
+    a.lse[at * a.q_heads + head] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945309f;
+  }
+}
+
+}  // namespace kv8
+
+// kv8_decode.cu: rows in groups of 8 to 32 on warp-level MMAs, for few rows per (sequence, kv head)
+void kv8_decode_plan(Kv8Attn& a, int sms);
+cudaError_t launch_kv8_decode(const Kv8Attn& a);
+// joins the chunks of a launch
+cudaError_t launch_kv8_combine(const Kv8Attn& a);
+inline size_t kv8_part_bytes(const Kv8Attn& a) {
+  if (a.chunks <= 1) return 0;
+  return static_cast<size_t>(a.seqs.batch) * a.pages.heads * a.row_groups * a.chunks * a.tile_rows * (a.head_dim + 2) *
+         sizeof(float);
+}
+
+}  // namespace qhtp

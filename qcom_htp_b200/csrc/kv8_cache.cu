@@ -1,0 +1,238 @@
+// Writing K and V rows into the 8-bit paged cache, and reading them back.
+//
+// A (block, kv head) tile of the cache has one float32 scale.  Per touched tile, with X the new rows
+// that fall into it (all arithmetic float32, every operation correctly rounded):
+//
+//   s_new = max|X| / 127, 0 below 2^-64, NaN if X holds a NaN or an infinity
+//   s     = s_new where the tile's slot 0 is written (the tile starts anew), else max(s_old, s_new),
+//           NaN if either is not finite
+//   new codes = clamp(rint(x * (1 / s)), -127, 127), 0 where s is 0 or NaN
+//   old codes = rint(c * (s_old / s)) where s grew
+//
+// One CTA owns one tile of K or of V, so a tile's scale, its old codes and its new ones are read and
+// written by that CTA alone: no atomics, and the same bytes in every run.
+//
+// Bound by memory: per element the input is read once (2 or 4 bytes) and one code byte is written; a
+// tile's rows stay in registers between the maximum and the rounding.
+#include "kv8.cuh"
+
+namespace qhtp {
+namespace kv8 {
+namespace {
+
+constexpr int kMaxThreads = 256;
+
+struct MoveArgs {
+  Pages pages;
+  Seqs seqs;
+  const int32_t* first;
+  Rows row[2];   // K, V
+  int vec_log2;  // 16-byte vectors of a row
+};
+
+// One CTA per (block of the sequence, K or V of a head, sequence).  NV: vectors a thread keeps in
+// registers; tiles with more than NV per thread read their rows a second time (from L2).
+template <typename T, int NV>
+__global__ void __launch_bounds__(kMaxThreads) kv8_write_kernel(const MoveArgs a) {
+  constexpr int VN = Vec<T>::n;
+  const int b = blockIdx.z, h = blockIdx.y >> 1, kv = blockIdx.y & 1;
+  long long row0;
+  const int n = seq_rows(a.seqs, b, row0);
+  const long long past = max(a.first[b], 0);
+  const int bs_log2 = a.pages.bs_log2, bs = 1 << bs_log2;
+  const long long blk = (past >> bs_log2) + blockIdx.x;
+  const long long lo = max(past, blk << bs_log2), hi = min(past + n, (blk + 1) << bs_log2);
+  if (lo >= hi) return;
+  const long long id = block_of(a.seqs, a.pages, b, blk);
+  if (id < 0) return;
+  const int slot0 = static_cast<int>(lo - (blk << bs_log2)), rows = static_cast<int>(hi - lo);
+
+  const Rows& src = a.row[kv];
+  const T* x = static_cast<const T*>(src.data) + b * src.batch_stride + (row0 + lo - past) * src.token_stride +
+               h * src.head_stride;
+  const long long tile = id * a.pages.heads + h;
+  const int d = VN << a.vec_log2;
+  int8_t* codes = (kv ? a.pages.v : a.pages.k) + tile * bs * d;
+  float* scale_at = (kv ? a.pages.v_scale : a.pages.k_scale) + tile;
+  const float old = slot0 ? *scale_at : 0.0f;
+
+  const int nvec = rows << a.vec_log2, cmask = (1 << a.vec_log2) - 1;
+  auto load = [&](int i) {
+    return __ldg(reinterpret_cast<const uint4*>(x + (i >> a.vec_log2) * src.token_stride + (i & cmask) * VN));
+  };
+  uint4 raw[NV];
+  uint32_t top = 0;  // max |x| as bits: ordered like the values, infinity and NaN above all of them
+  auto take = [&](const uint4& r) {
+    float f[VN];
+    Vec<T>::load(r, f);
+#pragma unroll
+    for (int e = 0; e < VN; ++e) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
+  };
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int at = threadIdx.x + i * blockDim.x;
+    raw[i] = at < nvec ? load(at) : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) take(raw[i]);
+  for (int at = threadIdx.x + NV * blockDim.x; at < nvec; at += blockDim.x) take(load(at));
+
+  __shared__ uint32_t s_top[kMaxThreads / 32];
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
+  __syncthreads();  // also: every thread has read the old scale
+  for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) top = max(top, s_top[w]);
+
+  float s = __fdiv_rn(__uint_as_float(top), 127.0f);
+  if (s < kScaleMin) s = 0.0f;
+  if (slot0) s = fmaxf(s, old);  // fmaxf drops a NaN: both are looked at below
+  const bool fine = top < 0x7f800000u && isfinite(old);
+  if (!fine) s = nan_f32();
+  if (threadIdx.x == 0) *scale_at = s;
+  const float inv = fine && s > 0.0f ? __frcp_rn(s) : 0.0f;
+
+  auto put = [&](int at, const uint4& r) {
+    float f[VN];
+    Vec<T>::load(r, f);
+    uint32_t w[VN / 4];
+#pragma unroll
+    for (int e = 0; e < VN / 4; ++e) {
+      uint32_t c[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // with inv 0 a NaN or infinity gives NaN here; fminf / fmaxf then return a bound
+        const float q = fminf(fmaxf(rintf(__fmul_rn(f[4 * e + j], inv)), -127.0f), 127.0f);
+        c[j] = fine ? static_cast<uint32_t>(__float2int_rn(q)) : 0u;
+      }
+      w[e] = prmt(prmt(c[0], c[1], 0x0040u), prmt(c[2], c[3], 0x0040u), 0x5410u);
+    }
+    int8_t* to = codes + ((slot0 << a.vec_log2) + at) * VN;
+    if constexpr (VN == 8)
+      *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+    else
+      *reinterpret_cast<uint32_t*>(to) = w[0];
+  };
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int at = threadIdx.x + i * blockDim.x;
+    if (at < nvec) put(at, raw[i]);
+  }
+  for (int at = threadIdx.x + NV * blockDim.x; at < nvec; at += blockDim.x) put(at, load(at));
+
+  if (slot0 == 0 || !fine || s == old) return;
+  // the scale grew: what the tile held before, in the new scale
+  const float ratio = __fdiv_rn(old, s);
+  const int words = slot0 * d / 16;
+  uint4* held = reinterpret_cast<uint4*>(codes);
+  for (int i = threadIdx.x; i < words; i += blockDim.x) {
+    const uint4 r = held[i];
+    uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      uint32_t c[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        c[j] = static_cast<uint32_t>(
+            __float2int_rn(__fmul_rn(static_cast<float>(static_cast<int8_t>(w[e] >> (8 * j))), ratio)));
+      w[e] = prmt(prmt(c[0], c[1], 0x0040u), prmt(c[2], c[3], 0x0040u), 0x5410u);
+    }
+    held[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// One CTA per (block of the sequence, K or V of a head, sequence), 16 codes a thread and step.  Rows whose block the table does not map come back as NaN.
+template <typename T>
+__global__ void __launch_bounds__(kMaxThreads) kv8_read_kernel(const MoveArgs a) {
+  constexpr int VN = Vec<T>::n;
+  const int b = blockIdx.z, h = blockIdx.y >> 1, kv = blockIdx.y & 1;
+  long long row0;
+  const int n = seq_rows(a.seqs, b, row0);
+  const long long past = a.first[b];
+  const int bs_log2 = a.pages.bs_log2;
+  const long long blk = (past >> bs_log2) + blockIdx.x;
+  const long long lo = max(past, blk << bs_log2), hi = min(past + n, (blk + 1) << bs_log2);
+  if (lo >= hi) return;
+  const long long id = block_of(a.seqs, a.pages, b, blk);
+  const int slot0 = static_cast<int>(lo - (blk << bs_log2)), rows = static_cast<int>(hi - lo);
+  const int d = 16 << a.vec_log2;
+  const long long tile = max(id, 0ll) * a.pages.heads + h;
+  const int8_t* codes = (kv ? a.pages.v : a.pages.k) + ((tile << bs_log2) + slot0) * d;
+  const float s = id < 0 ? nan_f32() : (kv ? a.pages.v_scale : a.pages.k_scale)[tile];
+  const Rows& dst = a.row[kv];
+  T* x = static_cast<T*>(dst.data) + b * dst.batch_stride + (row0 + lo - past) * dst.token_stride + h * dst.head_stride;
+  const int nvec = rows << a.vec_log2, cmask = (1 << a.vec_log2) - 1;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < nvec; i += blockDim.x) {
+    const uint4 r = __ldg(reinterpret_cast<const uint4*>(codes) + i);
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+    T* to = x + (i >> a.vec_log2) * dst.token_stride + (i & cmask) * 16;
+#pragma unroll
+    for (int e = 0; e < 16 / VN; ++e) {
+      float f[VN];
+#pragma unroll
+      for (int j = 0; j < VN; ++j) {
+        const int at = e * VN + j;
+        f[j] = __fmul_rn(static_cast<float>(static_cast<int8_t>(w[at >> 2] >> (8 * (at & 3)))), s);
+      }
+      *reinterpret_cast<uint4*>(to + e * VN) = Vec<T>::store(f);
+    }
+  }
+}
+
+// Blocks that the rows of one sequence can touch.
+unsigned blocks_touched(const Kv8Move& m) {
+  const long long bs = 1ll << m.pages.bs_log2;
+  return static_cast<unsigned>((m.seqs.tokens + bs - 2) / bs + 1);
+}
+
+int log2_of(int x) {
+  int l = 0;
+  while ((1 << l) < x) ++l;
+  return l;
+}
+
+template <typename T>
+cudaError_t write(const Kv8Move& m) {
+  MoveArgs a{m.pages, m.seqs, m.first, {m.k, m.v}, log2_of(m.head_dim / Vec<T>::n)};
+  const dim3 grid(blocks_touched(m), 2 * m.pages.heads, m.seqs.batch);
+  const int rows = m.seqs.tokens < (1 << m.pages.bs_log2) ? m.seqs.tokens : 1 << m.pages.bs_log2;
+  const int vecs = rows * m.head_dim / Vec<T>::n;
+  // four vectors a thread where the tile has them: enough loads in flight per thread, and 128 threads
+  // at the least, for the tiles of single tokens whose old codes have to be scaled anew
+  const int threads = vecs >= 4 * 256 ? 256 : 128;
+  const int per = (vecs + threads - 1) / threads;
+  if (per <= 1)
+    kv8_write_kernel<T, 1><<<grid, threads, 0, m.stream>>>(a);
+  else if (per <= 4)
+    kv8_write_kernel<T, 4><<<grid, threads, 0, m.stream>>>(a);
+  else
+    kv8_write_kernel<T, 8><<<grid, threads, 0, m.stream>>>(a);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t read(const Kv8Move& m) {
+  MoveArgs a{m.pages, m.seqs, m.first, {m.k, m.v}, log2_of(m.head_dim / 16)};
+  const dim3 grid(blocks_touched(m), 2 * m.pages.heads, m.seqs.batch);
+  const int rows = m.seqs.tokens < (1 << m.pages.bs_log2) ? m.seqs.tokens : 1 << m.pages.bs_log2;
+  const int vecs = rows * m.head_dim / 16;
+  kv8_read_kernel<T><<<grid, vecs >= 512 ? 256 : 128, 0, m.stream>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+}  // namespace kv8
+
+cudaError_t launch_kv8_write(const Kv8Move& m) {
+  if (m.dtype == QHTP_DTYPE_BF16) return kv8::write<__nv_bfloat16>(m);
+  if (m.dtype == QHTP_DTYPE_F16) return kv8::write<__half>(m);
+  return kv8::write<float>(m);
+}
+
+cudaError_t launch_kv8_read(const Kv8Move& m) {
+  if (m.dtype == QHTP_DTYPE_BF16) return kv8::read<__nv_bfloat16>(m);
+  if (m.dtype == QHTP_DTYPE_F16) return kv8::read<__half>(m);
+  return kv8::read<float>(m);
+}
+
+}  // namespace qhtp

@@ -1,0 +1,477 @@
+// Attention of few query rows (single tokens, drafted tokens) over the 8-bit paged KV cache.
+//
+// Per row:  t_j = q . ck_j * (scale log2(e) sk) + log2(sv),   p_j = 2^(t_j - m),   m the running maximum of t
+//           out = sum_j p_j cv_j / sum_j p_j / sv,            lse = ln 2 (m + log2(sum_j p_j / sv))
+// with ck, cv the int8 codes of key j and sk, sv the scales of its block.  V's scale enters the
+// exponent, so the codes themselves are the tensor core's operands (int8 is exact in f16), a scale
+// costs nothing per element, and since the maximum is taken over t the largest p is 1: p rounded to f16
+// loses at most 2^-12 of what it adds to the output.  Scores, maxima, sums and outputs are float32.
+//
+// Bound by memory: two bytes per key and element.  The keys of a (sequence, kv head) are cut into chunks
+// over the grid; a CTA's four warps take 32 keys in turn, straight from global memory to registers in
+// 16-byte loads (a block's tile of a head is contiguous), K of the next step while the softmax of this
+// one runs.  Keys are the M side of the MMAs (m16n8k16, S^T = K Q^T and O^T = V^T P^T), so a group of
+// eight query rows wastes nothing; which head_dim index a fragment's k stands for is free, and is chosen
+// so that a thread's 16 loaded bytes are its fragments.
+#include <algorithm>
+
+#include "kv8.cuh"
+
+namespace qhtp {
+namespace kv8 {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kSeg = 2048;                  // keys whose block constants are in shared memory
+constexpr int kSegBlocks = kSeg / 16 + 2;
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Transpose of an 8x8 matrix of 16-bit values held as one row pair per thread.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// NT groups of eight rows; K16 groups of 16 keys per step.
+template <int D, int NT, int K16>
+__global__ void __launch_bounds__(kWarps * 32) kv8_decode_kernel(const Kv8Attn a) {
+  constexpr int kRows = 8 * NT;
+  constexpr int kQStride = D + 4;      // halves: rows 2 banks apart, so the 64-bit fragment reads do not collide
+  constexpr int kOStride = D + 4;
+  constexpr int KJ = D / 64;           // 16-byte pieces of a key in one thread
+  constexpr int VW = D / 32;           // words of a V row in one thread
+  constexpr int MT = D / 16;
+  __shared__ __align__(16) __half s_q[kRows * kQStride];
+  __shared__ __align__(16) float s_o[kRows * kOStride];
+  __shared__ float s_down[kRows], s_m[kWarps][kRows], s_l[kWarps][kRows];
+  __shared__ int s_lo[kRows], s_hi[kRows];
+  __shared__ long long s_off[kSegBlocks];
+  __shared__ float s_c[kSegBlocks], s_lw[kSegBlocks], s_iw[kSegBlocks];
+
+  const int b = blockIdx.z, h = blockIdx.y, rg = blockIdx.x / a.chunks, chunk = blockIdx.x - rg * a.chunks;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
+  long long row0;
+  const int T = seq_rows(a.seqs, b, row0);
+  const int R = T * a.group, r0 = rg * kRows;
+  if (r0 >= R) return;
+  const int r1 = min(R, r0 + kRows);
+  const int len = seq_length(a, b);
+  const Span all = row_span(a, len, T, r0, r1);
+  const Span keys = chunk_span(a, all, chunk);
+  // an empty chunk leaves nothing; where every chunk is empty, the first one writes the rows
+  if (keys.lo >= keys.hi && chunk > 0) return;
+  // each row of the group sees the keys [all_lo, all_hi)
+  const int all_hi = a.causal ? len - T + r0 / a.group + 1 : len;
+  const int all_lo = a.window ? len - T + (r1 - 1) / a.group - a.window + 1 : 0;
+
+  // the rows of q, each scaled by a power of two into f16
+  for (int r = warp; r < kRows; r += kWarps) {
+    constexpr int E = D / 32;  // elements of a lane
+    float x[E];
+    const int row = r0 + r;
+    const bool live = row < r1;
+    if (live) {
+      const long long at = b * a.q.batch_stride + (row0 + row / a.group) * a.q.token_stride +
+                           (static_cast<long long>(h) * a.group + row % a.group) * a.q.head_stride + lane * E;
+      const uint16_t* src = static_cast<const uint16_t*>(a.q.data) + at;
+      uint32_t w[(E + 1) / 2];
+      if constexpr (E == 8) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(src));
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+      } else if constexpr (E == 4) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(src));
+        w[0] = v.x, w[1] = v.y;
+      } else {
+        w[0] = __ldg(reinterpret_cast<const uint32_t*>(src));
+      }
+#pragma unroll
+      for (int i = 0; i < E / 2; ++i) {
+        if (a.bf16) {
+          x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        } else {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+          x[2 * i] = f.x, x[2 * i + 1] = f.y;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) x[i] = 0.0f;
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+    top = __reduce_max_sync(0xffffffffu, top);
+    float up, down;
+    row_factor(__uint_as_float(top), up, down);
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i)
+      *reinterpret_cast<uint32_t*>(&s_q[r * kQStride + lane * E + 2 * i]) = pack_half2(x[2 * i] * up, x[2 * i + 1] * up);
+    if (lane == 0) {
+      const int p = len - T + row / a.group;
+      s_down[r] = down;
+      s_hi[r] = live ? (a.causal ? min(len, p + 1) : len) : 0;
+      s_lo[r] = a.window ? p - a.window + 1 : 0;
+    }
+  }
+  __syncthreads();
+
+  float acc[NT][MT][4], m[NT][2], l[NT][2], f[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) m[n][i] = -INFINITY, l[n][i] = 0.0f, f[n][i] = s_down[8 * n + 2 * q4 + i];
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[n][t][i] = 0.0f;
+  }
+
+  const int bs_log2 = a.pages.bs_log2, bs = 1 << bs_log2;
+  for (int seg = keys.lo; seg < keys.hi; seg += kSeg) {
+    const int seg_hi = min(keys.hi, seg + kSeg);
+    const int blk0 = seg >> bs_log2, nblk = ((seg_hi - 1) >> bs_log2) - blk0 + 1;
+    for (int i = threadIdx.x; i < nblk; i += kWarps * 32) {
+      const long long id = block_of(a.seqs, a.pages, b, blk0 + i);
+      s_off[i] = ((max(id, 0ll) * a.pages.heads + h) << bs_log2) * D;
+      const BlockScales s = block_scales(a, id, h);
+      s_c[i] = s.c, s_lw[i] = s.log2_w, s_iw[i] = s.inv_w;
+    }
+    __syncthreads();
+
+    const int groups = (seg_hi - seg + 15) >> 4, tiles = (groups + K16 - 1) / K16;
+    uint4 kr[K16][2][KJ];
+    uint32_t vr[K16][4][VW];
+    auto place = [&](int gi, long long& off) {  // block index in the segment, and the group's first code
+      const int key = seg + min(gi, groups - 1) * 16, bi = (key >> bs_log2) - blk0;
+      off = s_off[bi] + static_cast<long long>(key & (bs - 1)) * D;
+      return bi;
+    };
+    auto load_k = [&](int tile) {
+#pragma unroll
+      for (int i = 0; i < K16; ++i) {
+        long long off;
+        place(tile * K16 + i, off);
+        const int8_t* p = a.pages.k + off + g * D + 16 * q4;
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) {
+          kr[i][0][j] = __ldg(reinterpret_cast<const uint4*>(p + 64 * j));
+          kr[i][1][j] = __ldg(reinterpret_cast<const uint4*>(p + 8 * D + 64 * j));
+        }
+      }
+    };
+    auto load_v = [&](int tile) {
+#pragma unroll
+      for (int i = 0; i < K16; ++i) {
+        long long off;
+        place(tile * K16 + i, off);
+        const int8_t* p = a.pages.v + off + (D / 8) * g;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int8_t* row = p + (2 * q4 + (x & 1) + 8 * (x >> 1)) * D;
+          if constexpr (VW == 2) {
+            const uint2 v = __ldg(reinterpret_cast<const uint2*>(row));
+            vr[i][x][0] = v.x, vr[i][x][1] = v.y;
+          } else {
+#pragma unroll
+            for (int w = 0; w < VW; w += 4) {
+              const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + 4 * w));
+              vr[i][x][w] = v.x, vr[i][x][w + 1] = v.y, vr[i][x][w + 2] = v.z, vr[i][x][w + 3] = v.w;
+            }
+          }
+        }
+      }
+    };
+    if (warp < tiles) {
+      load_k(warp);
+      load_v(warp);
+    }
+    for (int tile = warp; tile < tiles; tile += kWarps) {
+      // S^T = K Q^T
+      float s[K16][NT][4];
+#pragma unroll
+      for (int i = 0; i < K16; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[i][n][e] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < KJ; ++j) {
+#pragma unroll
+        for (int st = 0; st < 4; ++st) {
+          uint2 qf[NT];
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            qf[n] = *reinterpret_cast<const uint2*>(&s_q[(8 * n + g) * kQStride + 64 * j + 16 * q4 + 4 * st]);
+#pragma unroll
+          for (int i = 0; i < K16; ++i) {
+            const uint32_t w0 = reinterpret_cast<const uint32_t*>(&kr[i][0][j])[st];
+            const uint32_t w1 = reinterpret_cast<const uint32_t*>(&kr[i][1][j])[st];
+            uint32_t a0, a1, a2, a3;
+            codes_to_half2(w0, a0, a2);
+            codes_to_half2(w1, a1, a3);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_f16(s[i][n], a0, a1, a2, a3, qf[n].x, qf[n].y);
+          }
+        }
+      }
+      if (tile + kWarps < tiles) load_k(tile + kWarps);
+
+      const int key0 = seg + tile * 16 * K16;
+      const bool masked = key0 + 16 * K16 > all_hi || key0 < all_lo;
+      float iw[K16], top[NT][2];
+      bool zero[K16];  // a tile of V whose scale counts as zero
+#pragma unroll
+      for (int n = 0; n < NT; ++n) top[n][0] = m[n][0], top[n][1] = m[n][1];
+#pragma unroll
+      for (int i = 0; i < K16; ++i) {
+        long long off;
+        const int bi = place(tile * K16 + i, off);
+        const float c = s_c[bi], lw = s_lw[bi];
+        iw[i] = s_iw[bi];
+        zero[i] = iw[i] == kZeroTile;
+        if (zero[i]) iw[i] *= 0.5f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float t = fmaf(s[i][n][e], c * f[n][e & 1], lw);
+            if (masked) {
+              const int key = key0 + 16 * i + g + 8 * (e >> 1), r = 8 * n + 2 * q4 + (e & 1);
+              if (key >= s_hi[r] || key < s_lo[r]) t = -INFINITY;
+            }
+            s[i][n][e] = t;
+            top[n][e & 1] = fmaxf(top[n][e & 1], t);
+          }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) top[n][i] = fmaxf(top[n][i], __shfl_xor_sync(0xffffffffu, top[n][i], x));
+          // a row that has seen nothing yet keeps the maximum -inf; its terms are 2^-inf against 0
+          const float base = top[n][i] == -INFINITY ? 0.0f : top[n][i];
+          const float alpha = ex2(m[n][i] - base);
+          m[n][i] = top[n][i];
+          top[n][i] = base;
+          l[n][i] *= alpha;
+#pragma unroll
+          for (int t = 0; t < MT; ++t) acc[n][t][i] *= alpha, acc[n][t][i + 2] *= alpha;
+        }
+      uint32_t pb[K16][NT][2];
+#pragma unroll
+      for (int i = 0; i < K16; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float p[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            p[e] = ex2(s[i][n][e] - top[n][e & 1]);
+            // a masked key adds nothing, whatever its block's scale is
+            l[n][e & 1] += masked && p[e] == 0.0f ? 0.0f : p[e] * iw[i];
+          }
+          pb[i][n][0] = transpose8(zero[i] ? 0u : pack_half2(p[0], p[1]));
+          pb[i][n][1] = transpose8(zero[i] ? 0u : pack_half2(p[2], p[3]));
+        }
+      // O^T += V^T P^T
+#pragma unroll
+      for (int i = 0; i < K16; ++i) {
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+          uint32_t x[2][4];  // [key pair][element of the word]
+#pragma unroll
+          for (int kp = 0; kp < 2; ++kp) {
+            const uint32_t u0 = vr[i][2 * kp][w] ^ 0x80808080u, u1 = vr[i][2 * kp + 1][w] ^ 0x80808080u;
+            const uint32_t lo = prmt(u0, u1, 0x5140u), hi = prmt(u0, u1, 0x7362u);
+            x[kp][0] = sub_1152(prmt(lo, 0x64646464u, 0x4140u));
+            x[kp][1] = sub_1152(prmt(lo, 0x64646464u, 0x4342u));
+            x[kp][2] = sub_1152(prmt(hi, 0x64646464u, 0x4140u));
+            x[kp][3] = sub_1152(prmt(hi, 0x64646464u, 0x4342u));
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma_f16(acc[n][2 * w], x[0][0], x[0][1], x[1][0], x[1][1], pb[i][n][0], pb[i][n][1]);
+            mma_f16(acc[n][2 * w + 1], x[0][2], x[0][3], x[1][2], x[1][3], pb[i][n][0], pb[i][n][1]);
+          }
+        }
+      }
+      if (tile + kWarps < tiles) load_v(tile + kWarps);
+    }
+    __syncthreads();  // the segment's constants are read
+  }
+
+  // join the warps: every row's maximum, then the rows added up one warp after the other
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], x);
+      if (g == 0) s_m[warp][8 * n + 2 * q4 + i] = m[n][i], s_l[warp][8 * n + 2 * q4 + i] = l[n][i];
+    }
+  __syncthreads();
+  for (int w = 0; w < kWarps; ++w) {
+    if (warp == w) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = 8 * n + 2 * q4 + i;
+          float top = s_m[0][r];
+#pragma unroll
+          for (int x = 1; x < kWarps; ++x) top = fmaxf(top, s_m[x][r]);
+          const float alpha = ex2(m[n][i] - (top == -INFINITY ? 0.0f : top));
+          float* o = s_o + r * kOStride + (D / 8) * g;
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            const float x0 = acc[n][t][i] * alpha, x1 = acc[n][t][i + 2] * alpha;
+            o[2 * t] = w ? o[2 * t] + x0 : x0;
+            o[2 * t + 1] = w ? o[2 * t + 1] + x1 : x1;
+          }
+        }
+    }
+    __syncthreads();
+  }
+
+  const long long part = part_row(a, b, h, rg, chunk);
+  for (int i = threadIdx.x; i < kRows * (D / 8); i += kWarps * 32) {
+    const int r = i / (D / 8), c = i - r * (D / 8), row = r0 + r;
+    if (row >= r1) break;
+    float top = s_m[0][r];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) top = fmaxf(top, s_m[w][r]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) sum += s_l[w][r] * ex2(s_m[w][r] - base);
+    float o[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = s_o[r * kOStride + 8 * c + e];
+    if (a.chunks == 1) {
+      write_row8(a, b, row0, row, h, 8 * c, o, sum, base);
+    } else {
+      float4* to = reinterpret_cast<float4*>(a.part + (part + r) * D + 8 * c);
+      to[0] = make_float4(o[0], o[1], o[2], o[3]);
+      to[1] = make_float4(o[4], o[5], o[6], o[7]);
+      if (c == 0) {
+        float* ml = a.part + part_rows(a) * D + 2 * (part + r);
+        ml[0] = base, ml[1] = sum;
+      }
+    }
+  }
+}
+
+// The chunks of each row joined: D / 8 threads a row, 128 / (D / 8) rows of a (sequence, kv head) a CTA.
+template <int D>
+__global__ void __launch_bounds__(128) kv8_combine_kernel(const Kv8Attn a) {
+  constexpr int kLanes = D / 8;                 // threads of a row
+  constexpr int kPer = 128 / kLanes;            // rows of a CTA
+  griddep_wait();
+  const int b = blockIdx.z, h = blockIdx.y, row = blockIdx.x * kPer + threadIdx.x / kLanes, c = threadIdx.x % kLanes;
+  long long row0;
+  const int T = seq_rows(a.seqs, b, row0);
+  const int R = T * a.group, rg = row / a.tile_rows, r0 = rg * a.tile_rows, r1 = min(R, r0 + a.tile_rows), r = row - r0;
+  if (row >= R || rg >= a.row_groups) return;
+  const Span all = row_span(a, seq_length(a, b), T, r0, r1);
+  int n = 1;
+  while (n < a.chunks && chunk_span(a, all, n).lo < chunk_span(a, all, n).hi) ++n;
+  const long long part = part_row(a, b, h, rg, 0) + r;
+  const float* ml = a.part + part_rows(a) * D;
+  float top = -INFINITY;
+  for (int i = 0; i < n; ++i) {
+    const long long p = part + static_cast<long long>(i) * a.tile_rows;
+    if (ml[2 * p + 1] != 0.0f) top = fmaxf(top, ml[2 * p]);
+  }
+  if (top == -INFINITY) top = 0.0f;
+  float sum = 0.0f, o[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const long long p = part + static_cast<long long>(i) * a.tile_rows;
+    const float l = ml[2 * p + 1];
+    const float f = l != 0.0f ? ex2(ml[2 * p] - top) : 0.0f;
+    const float4* x = reinterpret_cast<const float4*>(a.part + p * D + 8 * c);
+    const float4 u = x[0], v = x[1];
+    sum = fmaf(l, f, sum);
+    o[0] = fmaf(u.x, f, o[0]), o[1] = fmaf(u.y, f, o[1]), o[2] = fmaf(u.z, f, o[2]), o[3] = fmaf(u.w, f, o[3]);
+    o[4] = fmaf(v.x, f, o[4]), o[5] = fmaf(v.y, f, o[5]), o[6] = fmaf(v.z, f, o[6]), o[7] = fmaf(v.w, f, o[7]);
+  }
+  write_row8(a, b, row0, row, h, 8 * c, o, sum, top);
+}
+
+template <int D, int NT, int K16>
+cudaError_t run(const Kv8Attn& a) {
+  const dim3 grid(static_cast<unsigned>(a.chunks) * a.row_groups, a.pages.heads, a.seqs.batch);
+  kv8_decode_kernel<D, NT, K16><<<grid, kWarps * 32, 0, a.stream>>>(a);
+  return cudaGetLastError();
+}
+
+template <int D>
+cudaError_t combine(const Kv8Attn& a) {
+  const int per = 128 / (D / 8);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<long long>(a.seqs.tokens) * a.group + per - 1) / per), a.pages.heads, a.seqs.batch);
+  cfg.blockDim = dim3(128);
+  cfg.stream = a.stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv8_combine_kernel<D>, a);
+}
+
+}  // namespace
+}  // namespace kv8
+
+void kv8_decode_plan(Kv8Attn& a, int sms) {
+  const long long rows = static_cast<long long>(a.seqs.tokens) * a.group;
+  const int most = a.head_dim == 256 ? 16 : 32;
+  a.tile_rows = rows <= 8 ? 8 : rows <= 16 || most == 16 ? 16 : 32;
+  a.row_groups = static_cast<int>((rows + a.tile_rows - 1) / a.tile_rows);
+  const long long tiles = static_cast<long long>(a.seqs.batch) * a.pages.heads * a.row_groups;
+  // keys that a row group can see
+  long long span = a.max_len;
+  if (a.window) span = std::min(span, static_cast<long long>(a.window) + a.tile_rows + 31);
+  span = std::max(span, 1ll);
+  // Chunks fill three CTAs an SM twice over, of 256 keys at the least and 2048 at the most: the larger the
+  // chunk the less is spent on its start and its join, the smaller the better sequences of unlike lengths
+  // share the SMs.
+  long long chunk = (span * tiles + 6ll * sms - 1) / (6ll * sms);
+  chunk = (std::max(256ll, std::min(2048ll, chunk)) + 127) / 128 * 128;
+  a.chunks = static_cast<int>((span + chunk - 1) / chunk);
+  a.chunk = static_cast<int>(chunk);
+}
+
+cudaError_t launch_kv8_decode(const Kv8Attn& a) {
+  switch (a.head_dim * 100 + a.tile_rows) {
+    case 6408: return kv8::run<64, 1, 2>(a);
+    case 6416: return kv8::run<64, 2, 2>(a);
+    case 6432: return kv8::run<64, 4, 2>(a);
+    case 12808: return kv8::run<128, 1, 2>(a);
+    case 12816: return kv8::run<128, 2, 2>(a);
+    case 12832: return kv8::run<128, 4, 1>(a);
+    case 25608: return kv8::run<256, 1, 1>(a);
+    case 25616: return kv8::run<256, 2, 1>(a);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+cudaError_t launch_kv8_combine(const Kv8Attn& a) {
+  if (a.head_dim == 64) return kv8::combine<64>(a);
+  if (a.head_dim == 128) return kv8::combine<128>(a);
+  return kv8::combine<256>(a);
+}
+
+}  // namespace qhtp
