@@ -419,6 +419,11 @@ typedef struct QhtpKv8Attention {
 size_t qhtp_kv8_attention_workspace_bytes(const QhtpKv8Attention *run);
 QhtpStatus qhtp_kv8_attention(const QhtpKv8Attention *run);
 
+/* Synchronize `stream` and read (and clear) the current device's error word of qhtp_kv8_attention: non-zero
+ * (in *device_code if non-NULL), and QHTP_STATUS_RUNTIME_ERROR, after a wait inside a kernel gave up, which leaves
+ * the outputs of that call undefined. */
+QhtpStatus qhtp_kv8_check(int *device_code, void *stream);
+
 /* ------------------------------------------------------------------------------------------
  * Host-only helpers (no GPU needed).
  * ------------------------------------------------------------------------------------------ */

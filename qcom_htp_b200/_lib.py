@@ -145,6 +145,7 @@ SIGNATURES = {
     "qhtp_kv8_read": (C.c_int, [C.c_void_p]),
     "qhtp_kv8_attention_workspace_bytes": (C.c_size_t, [C.c_void_p]),
     "qhtp_kv8_attention": (C.c_int, [C.c_void_p]),
+    "qhtp_kv8_check": (C.c_int, [C.POINTER(C.c_int), C.c_void_p]),
     "qhtp_requant_code_host": (C.c_int32, [C.c_int64, C.c_uint64, C.c_int32, C.c_uint32, C.c_int32, C.c_uint64,
                                            C.c_uint64, C.c_int32, C.c_int32, C.c_int32]),
 }

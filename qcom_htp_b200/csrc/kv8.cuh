@@ -159,6 +159,7 @@ struct Kv8Attn {
   int causal, window;     // window 0: none
   float scale_log2;       // softmax scale * log2(e)
   int max_len;            // the caller's bound on the lengths (sizes the grid only)
+  int prompt;             // kv8_prompt.cu, else kv8_decode.cu
   // a launch's plan: rows per CTA, row groups of a sequence, keys per chunk, chunks
   int tile_rows, row_groups, chunk, chunks;
   float* part;            // workspace (chunks > 1): unnormalised rows, then their maxima and sums
@@ -248,6 +249,10 @@ __device__ __forceinline__ void write_row8(const Kv8Attn& a, int b, long long ro
 // kv8_decode.cu: rows in groups of 8 to 32 on warp-level MMAs, for few rows per (sequence, kv head)
 void kv8_decode_plan(Kv8Attn& a, int sms);
 cudaError_t launch_kv8_decode(const Kv8Attn& a);
+// kv8_prompt.cu: rows in tiles of 128 or 256 on tcgen05
+void kv8_prompt_plan(Kv8Attn& a, int sms);
+cudaError_t launch_kv8_prompt(const Kv8Attn& a);
+cudaError_t kv8_read_error(int* code, cudaStream_t stream);
 // joins the chunks of a launch
 cudaError_t launch_kv8_combine(const Kv8Attn& a);
 inline size_t kv8_part_bytes(const Kv8Attn& a) {

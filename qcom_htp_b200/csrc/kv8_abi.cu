@@ -120,7 +120,13 @@ QhtpStatus plan_attention(const QhtpKv8Attention* run, Kv8Attn* a) {
     a->chunks = 1;
     return QHTP_STATUS_OK;
   }
-  kv8_decode_plan(*a, sm_count());
+  a->prompt = static_cast<long long>(a->seqs.tokens) * a->group > (a->head_dim == 256 ? 16 : 32);
+  if (a->prompt)
+    kv8_prompt_plan(*a, sm_count());
+  else
+    kv8_decode_plan(*a, sm_count());
+  if (a->prompt && a->row_groups > 65535) return unsupported("kv8: too many rows");
+  if (static_cast<long long>(a->chunks) * a->pages.heads > (1ll << 30)) return unsupported("kv8: too many chunks");
   if (static_cast<long long>(a->chunks) * a->row_groups > (1ll << 30)) return unsupported("kv8: too many rows");
   return QHTP_STATUS_OK;
 }
@@ -164,9 +170,19 @@ QhtpStatus qhtp_kv8_attention(const QhtpKv8Attention* run) {
   a.lse = run->lse;
   a.part = static_cast<float*>(run->workspace);
   a.stream = static_cast<cudaStream_t>(run->stream);
-  cudaError_t e = launch_kv8_decode(a);
+  cudaError_t e = a.prompt ? launch_kv8_prompt(a) : launch_kv8_decode(a);
   if (e == cudaSuccess && a.chunks > 1) e = launch_kv8_combine(a);
   return status_from_cuda(e);
+}
+
+QhtpStatus qhtp_kv8_check(int* device_code, void* stream) {
+  int code = 0;
+  const QhtpStatus st = status_from_cuda(kv8_read_error(&code, static_cast<cudaStream_t>(stream)));
+  if (st != QHTP_STATUS_OK) return st;
+  if (device_code != nullptr) *device_code = code;
+  if (code == 0) return QHTP_STATUS_OK;
+  set_last_message("kv8: a wait inside an attention kernel gave up");
+  return QHTP_STATUS_RUNTIME_ERROR;
 }
 
 }  // extern "C"

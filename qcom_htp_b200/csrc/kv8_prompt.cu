@@ -1,0 +1,574 @@
+// Attention of many query rows (prompts, pieces of prompts) over the 8-bit paged KV cache, on tcgen05.
+//
+// The mathematics is kv8_decode.cu's: exponents t = q . ck * (scale log2(e) sk) + log2(sv), outputs
+// sum 2^(t - m) cv / sum 2^(t - m) / sv, the int8 codes as f16 operands, V's scale in the exponent.
+//
+// A CTA owns SLOTS tiles of 128 query rows (the tokens and heads of one kv head's group, packed) and walks
+// over the keys 128 at a time:
+//   K and V converters (a warpgroup each) load codes from the paged cache to registers, one tile ahead, and
+//     write them as f16 into 128-byte-swizzled images [key][64 head_dim]: K-major for Q K^T, and the same
+//     bytes MN-major for P V;
+//   one thread issues the MMAs: S = Q K^T into tensor memory, O += P V with P read from tensor memory;
+//   a softmax warpgroup per slot, a thread per row: S from tensor memory, P back over it as f16.
+// SLOTS = 2: the two tiles take turns, one's softmax under the other's MMAs.  SLOTS = 1 (one tile's rows, or
+// head_dim 256, whose O fills tensor memory): two S buffers, the softmax of one key tile under the MMAs of
+// its neighbours.
+//
+// m is raised, and O rescaled, only when a row's maximum has grown by more than 2^8: p then stays below
+// 2^8, far inside f16, and most tiles leave O alone.
+#include <algorithm>
+
+#include "kv8.cuh"
+
+namespace qhtp {
+namespace kv8 {
+namespace {
+
+constexpr int kKeys = 128;             // keys of a tile
+constexpr int kPanel = 128 * 128;      // bytes of a [128 rows][64 f16] swizzled image
+constexpr float kGrow = 8.0f;          // log2 of how far p may pass 1 before m follows
+
+template <int D, int SLOTS>
+struct Shape {
+  static constexpr int panels = D / 64;
+  static constexpr int stage = panels * kPanel;                 // a K or V tile
+  static constexpr int stages = D == 256 ? 1 : 2;               // of K, and of V
+  static constexpr int smem = (SLOTS + 2 * stages) * stage + 1024;
+  static constexpr int threads = (SLOTS + 3) * 128;
+  // registers of a thread: at launch (the most that the threads leave room for), and by role; the roles' sum is the launch's
+  static constexpr int regs = SLOTS == 2 ? 96 : 128;
+  static constexpr int softmax_regs = SLOTS == 2 ? 144 : 184;
+  static constexpr int convert_regs = SLOTS == 2 ? 72 : 136;
+  static constexpr int mma_regs = SLOTS == 2 ? 48 : 56;
+  static_assert(SLOTS * softmax_regs + 2 * convert_regs + mma_regs <= (SLOTS + 3) * regs, "registers");
+  static constexpr int o_col = 256;                             // S buffers in columns 0..255
+  static_assert(o_col + SLOTS * D <= 512, "tensor memory");
+};
+
+struct Barriers {
+  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done, o_full[2], drained;
+};
+
+template <int N>
+__device__ __forceinline__ void reg_alloc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void reg_free() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+// (a.x * b + c, a.y * b + c) in one instruction
+__device__ __forceinline__ float2 fma2(float x, float y, float b, float c) {
+  float2 r;
+  asm("{\n\t.reg .b64 u, v, w, z;\n\t"
+      "mov.b64 u, {%2, %3};\n\tmov.b64 v, {%4, %4};\n\tmov.b64 w, {%5, %5};\n\t"
+      "fma.rn.f32x2 z, u, v, w;\n\t"
+      "mov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(x), "f"(y), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 u, v, z;\n\t"
+      "mov.b64 u, {%2, %3};\n\tmov.b64 v, {%4, %5};\n\t"
+      "add.rn.f32x2 z, u, v;\n\t"
+      "mov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+// 16-byte chunk c of row r in a swizzled image
+__device__ __forceinline__ uint32_t swizzled(int r, int c) {
+  return static_cast<uint32_t>(r * 128 + (((c ^ r) & 7) << 4));
+}
+
+// The rows of one slot, scaled by a power of two each, as f16 into its image.
+template <int D>
+__device__ __forceinline__ void load_q(const Kv8Attn& a, int b, int h, long long row0, int r0, int r1, uint8_t* img,
+                                       float* down_at, int warp, int lane) {
+  constexpr int E = D / 32;
+  constexpr int kBatch = 8;  // rows of a warp in flight
+  for (int base = 0; base < 32; base += kBatch) {
+    uint32_t w[kBatch][E / 2];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int row = r0 + warp * 32 + base + i;
+#pragma unroll
+      for (int e = 0; e < E / 2; ++e) w[i][e] = 0;
+      if (row < r1) {
+        const int t = row / a.group;
+        const uint16_t* src = static_cast<const uint16_t*>(a.q.data) + b * a.q.batch_stride +
+                              (row0 + t) * a.q.token_stride +
+                              (static_cast<long long>(h) * a.group + row - t * a.group) * a.q.head_stride + lane * E;
+        if constexpr (E == 8) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(src));
+          w[i][0] = v.x, w[i][1] = v.y, w[i][2] = v.z, w[i][3] = v.w;
+        } else if constexpr (E == 4) {
+          const uint2 v = __ldg(reinterpret_cast<const uint2*>(src));
+          w[i][0] = v.x, w[i][1] = v.y;
+        } else {
+          w[i][0] = __ldg(reinterpret_cast<const uint32_t*>(src));
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int r = warp * 32 + base + i;
+      float x[E];
+#pragma unroll
+      for (int e = 0; e < E / 2; ++e) {
+        if (a.bf16) {
+          x[2 * e] = __uint_as_float(w[i][e] << 16), x[2 * e + 1] = __uint_as_float(w[i][e] & 0xffff0000u);
+        } else {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i][e]));
+          x[2 * e] = f.x, x[2 * e + 1] = f.y;
+        }
+      }
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+      top = __reduce_max_sync(0xffffffffu, top);
+      float up, down;
+      row_factor(__uint_as_float(top), up, down);
+      const int byte = lane * E * 2;
+      uint8_t* to = img + (byte >> 7) * kPanel + swizzled(r, (byte & 127) >> 4) + (byte & 15);
+#pragma unroll
+      for (int e = 0; e < E / 2; ++e) reinterpret_cast<uint32_t*>(to)[e] = pack_half2(x[2 * e] * up, x[2 * e + 1] * up);
+      if (lane == 0) down_at[r] = down;
+    }
+  }
+}
+
+// The word that a wait of a kernel here, having given up, leaves its code in.
+__device__ int g_error;
+
+// mbar_wait for a whole warp: every lane goes on, or none does.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
+}
+
+template <int D, int SLOTS>
+__global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel(const Kv8Attn a) {
+  using S = Shape<D, SLOTS>;
+  int* const err = &g_error;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Barriers bar;
+  __shared__ uint32_t s_tmem;
+  __shared__ float s_down[SLOTS * 128];
+  __shared__ float4 s_scale[4][8];  // (c, log2 w, 1 / w) of a tile's 16-key groups, four tiles deep
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // heads fastest, the longest row groups (the last of a causal sequence) first
+  const int h = blockIdx.x / a.chunks, chunk = blockIdx.x - h * a.chunks, b = blockIdx.y,
+            rg = a.row_groups - 1 - blockIdx.z;
+  long long row0;
+  const int T = seq_rows(a.seqs, b, row0);
+  const int R = T * a.group, r0 = rg * SLOTS * 128;
+  if (r0 >= R) return;
+  const int r1 = min(R, r0 + SLOTS * 128);
+  const int len = seq_length(a, b);
+  const Span all = row_span(a, len, T, r0, r1);
+  const Span keys = chunk_span(a, all, chunk);
+  const int tiles = keys.lo < keys.hi ? (keys.hi - keys.lo + kKeys - 1) / kKeys : 0;
+  if (tiles == 0 && chunk > 0) return;
+
+  uint8_t* const smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint8_t* const q_img = smem;
+  uint8_t* const k_img = smem + SLOTS * S::stage;
+  uint8_t* const v_img = k_img + S::stages * S::stage;
+
+  constexpr int kConvK = SLOTS * 4, kConvV = kConvK + 4, kMma = kConvV + 4;  // first warps of the roles
+  if (warp == kMma) {
+    tmem_alloc(&s_tmem, 512);
+    if (lane == 0) {
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&bar.q_full[i], 128);
+        mbar_init(&bar.k_full[i], 128);
+        mbar_init(&bar.v_full[i], 128);
+        mbar_init(&bar.k_empty[i], 1);
+        mbar_init(&bar.v_empty[i], 1);
+        mbar_init(&bar.s_full[i], 2);  // the MMAs, and the issuing thread's own arrival
+        mbar_init(&bar.p_full[i], 128);
+        mbar_init(&bar.o_full[i], 1);
+      }
+      mbar_init(&bar.pv_done, 1);
+      mbar_init(&bar.drained, 1);
+      fence_barrier_init();
+    }
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+
+  if (warp < kConvK) {
+    // ------------------------------------------------------------------------------- softmax, a thread per row
+    reg_alloc<S::softmax_regs>();
+    const int slot = warp >> 2, wq = warp & 3, r = r0 + slot * 128 + wq * 32 + lane;
+    const int sr0 = r0 + slot * 128, sr1 = min(r1, sr0 + 128);  // the slot's rows (none: sr0 >= sr1)
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(wq * 32) << 16);
+    const uint32_t o_at = lanes + S::o_col + slot * D;
+    float m = -INFINITY, l = 0.0f;
+    if (tiles > 0 && sr0 < sr1) {
+      load_q<D>(a, b, h, row0, sr0, sr1, q_img + slot * S::stage, s_down + slot * 128, wq, lane);
+      fence_proxy_async_smem();
+      mbar_arrive(&bar.q_full[slot]);
+      __syncwarp();
+      const float down = s_down[slot * 128 + wq * 32 + lane];
+      const int p = len - T + r / a.group;
+      const int row_hi = r >= sr1 ? 0 : a.causal ? min(len, p + 1) : len, row_lo = a.window ? p - a.window + 1 : 0;
+      // every row of the slot sees the keys [all_lo, all_hi)
+      const int all_hi = a.causal ? len - T + sr0 / a.group + 1 : len;
+      const int all_lo = a.window ? len - T + (sr1 - 1) / a.group - a.window + 1 : 0;
+      for (int j = 0; j < tiles; ++j) {
+        const int buf = SLOTS == 2 ? slot : j & 1;
+        const uint32_t phase = SLOTS == 2 ? j & 1 : (j >> 1) & 1;
+        const uint32_t s_at = lanes + buf * 128;
+        if (!warp_wait(&bar.s_full[buf], phase, err, kErrTimeoutAccum)) break;
+        tc_fence_after();
+        const float4* sc = s_scale[j & 3];
+        const int key0 = keys.lo + j * kKeys;
+        const bool masked = key0 + kKeys > all_hi || key0 < all_lo;
+        const int hi = row_hi - key0, lo = row_lo - key0;  // visible columns [lo, hi)
+
+        // the row's maximum
+        float top = m;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t x[32];
+          tmem_ld32(s_at + 32 * c, x);
+          tmem_ld_wait();
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            float best = -INFINITY;
+            if (!masked) {
+#pragma unroll
+              for (int e = 0; e < 16; e += 2)
+                best = max3(best, __uint_as_float(x[16 * g + e]), __uint_as_float(x[16 * g + e + 1]));
+            } else {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const int col = 32 * c + 16 * g + e;
+                if (col < hi && col >= lo) best = fmaxf(best, __uint_as_float(x[16 * g + e]));
+              }
+            }
+            const float4 k = sc[2 * c + g];
+            if (best != -INFINITY) top = fmaxf(top, fmaf(best, k.x * down, k.y));
+          }
+        }
+        // raise m where it pays; rows of a warp move together
+        if (__any_sync(0xffffffffu, top > m + kGrow || (m == -INFINITY && top != -INFINITY))) {
+          const float alpha = m == -INFINITY ? 0.0f : ex2(m - top);
+          if (j > 0) {
+            if (SLOTS == 1 && !warp_wait(&bar.pv_done, (j - 1) & 1, err, kErrTimeoutAccum)) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t x[32];
+              tmem_ld32(o_at + 32 * c, x);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * alpha);
+              tmem_st32(o_at + 32 * c, x);
+            }
+            tmem_st_wait();
+          }
+          l *= alpha;
+          m = top;
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+        // p, its sum, and p as f16 over the columns of S that have been read
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t x[32], w[16];
+          tmem_ld32(s_at + 32 * c, x);
+          tmem_ld_wait();
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const float4 k = sc[2 * c + g];
+            const float f = k.x * down, off = k.y - base;
+            float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              float2 t = fma2(__uint_as_float(x[16 * g + e]), __uint_as_float(x[16 * g + e + 1]), f, off);
+              t.x = ex2(t.x), t.y = ex2(t.y);
+              if (masked) {
+                const int col = 32 * c + 16 * g + e;
+                t.x = col < hi && col >= lo ? t.x : 0.0f;
+                t.y = col + 1 < hi && col + 1 >= lo ? t.y : 0.0f;
+              }
+              sum = add2(sum, t);
+              w[8 * g + e / 2] = pack_half2(t.x, t.y);
+            }
+            const float add = sum.x + sum.y;
+            if (k.z == kZeroTile) {  // a tile of V whose scale counts as zero
+              l = fmaf(add, 0.5f * kZeroTile, l);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) w[8 * g + e] = 0;
+            } else if (!masked || add != 0.0f) {  // masked keys add nothing, whatever their scale is
+              l = fmaf(add, k.z, l);
+            }
+          }
+          tmem_st16(s_at + 16 * c, w);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&bar.p_full[buf]);
+      }
+      warp_wait(&bar.o_full[slot], 0, err, kErrTimeoutAccum);
+      tc_fence_after();
+    }
+    // the rows
+    if (sr0 < sr1) {
+      const float base = m == -INFINITY ? 0.0f : m;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const bool live = r < sr1;
+      const int t = r / a.group, head = h * a.group + r - t * a.group;
+      const long long part = part_row(a, b, h, rg, chunk) + slot * 128 + wq * 32 + lane;
+      uint16_t* out = static_cast<uint16_t*>(a.out.data) + b * a.out.batch_stride + (row0 + t) * a.out.token_stride +
+                      head * a.out.head_stride;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t x[32];
+        if (tiles > 0) {
+          tmem_ld32(o_at + 32 * c, x);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) x[e] = 0;
+        }
+        __syncwarp();
+        if (live && a.chunks == 1) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(x[e + i]) * inv;
+            *reinterpret_cast<uint4*>(out + 32 * c + e) = a.bf16 ? Vec<__nv_bfloat16>::store(v) : Vec<__half>::store(v);
+          }
+        } else if (live) {
+          uint4* to = reinterpret_cast<uint4*>(a.part + part * D + 32 * c);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) to[e] = make_uint4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+        }
+        __syncwarp();
+      }
+      if (live && a.chunks == 1 && a.lse != nullptr) {
+        const long long at = (a.seqs.start ? row0 : static_cast<long long>(b) * a.seqs.tokens) + t;
+        a.lse[at * a.q_heads + head] = l == 0.0f ? -INFINITY : (base + log2f(l)) * 0.693147180559945309f;
+      } else if (live && a.chunks > 1) {
+        float* ml = a.part + part_rows(a) * D + 2 * part;
+        ml[0] = base, ml[1] = l;
+      }
+    }
+  } else if (warp < kMma) {
+    // ------------------------------------------------------------------------------- codes to f16 images
+    if constexpr (S::convert_regs < S::regs) reg_free<S::convert_regs>(); else reg_alloc<S::convert_regs>();
+    const bool is_v = warp >= kConvV;
+    const int t = threadIdx.x - (is_v ? kConvV : kConvK) * 32;
+    constexpr int kPieces = D / 16;          // 16-code pieces of a key, and of a thread
+    const int8_t* const codes = is_v ? a.pages.v : a.pages.k;
+    uint64_t* const full = is_v ? bar.v_full : bar.k_full;
+    uint64_t* const empty = is_v ? bar.v_empty : bar.k_empty;
+    uint8_t* const img = is_v ? v_img : k_img;
+    const bool scales = warp == kConvK;      // this warp also brings the tiles' scales
+    const int bs_log2 = a.pages.bs_log2, bs = 1 << bs_log2;
+    const int piece = t % kPieces;
+    // block of the tile's 16-key group `lane` (of eight); -1: none
+    auto ids_of = [&](int j) {
+      const int key = keys.lo + j * kKeys + 16 * (lane & 7);
+      return j < tiles && key < keys.hi ? static_cast<int>(block_of(a.seqs, a.pages, b, key >> bs_log2)) : -1;
+    };
+    auto load = [&](int j, int ids, int i) {
+      const int k = i * (128 / kPieces) + t / kPieces;  // key of the tile
+      const int id = max(__shfl_sync(0xffffffffu, ids, k >> 4), 0);
+      const int slot = (keys.lo + j * kKeys + k) & (bs - 1);
+      return __ldg(reinterpret_cast<const uint4*>(
+          codes + ((((static_cast<long long>(id) * a.pages.heads + h) << bs_log2) + slot) * D + 16 * piece)));
+    };
+    uint4 raw[kPieces];
+    int ids = ids_of(0);
+    if (tiles > 0) {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) raw[i] = load(0, ids, i);
+    }
+    BlockScales sc{};
+    if (scales && tiles > 0) sc = block_scales(a, ids, h);
+    ids = ids_of(1);
+    for (int j = 0; j < tiles; ++j) {
+      const int st = j % S::stages;
+      if (j >= S::stages && !warp_wait(&empty[st], ((j / S::stages) - 1) & 1, err, kErrTimeoutEmpty)) break;
+      if (scales) {
+        if (lane < 8) s_scale[j & 3][lane] = make_float4(sc.c, sc.log2_w, sc.inv_w, 0.0f);
+        sc = block_scales(a, ids, h);
+      }
+      uint8_t* const to = img + st * S::stage;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const uint4 x = raw[i];
+        if (j + 1 < tiles) raw[i] = load(j + 1, ids, i);
+        const int k = i * (128 / kPieces) + t / kPieces;
+        uint32_t u[8];
+        codes_to_half2(x.x, u[0], u[1]);
+        codes_to_half2(x.y, u[2], u[3]);
+        codes_to_half2(x.z, u[4], u[5]);
+        codes_to_half2(x.w, u[6], u[7]);
+        const uint4 lo = make_uint4(u[0], u[1], u[2], u[3]), hi = make_uint4(u[4], u[5], u[6], u[7]);
+        uint8_t* const panel = to + (piece >> 2) * kPanel;
+        const int c = 2 * (piece & 3);
+        // eight threads of a store fill eight different chunks: every other panel starts with the odd ones
+        const bool odd = (piece >> 2) & 1;
+        *reinterpret_cast<uint4*>(panel + swizzled(k, c + (odd ? 1 : 0))) = odd ? hi : lo;
+        *reinterpret_cast<uint4*>(panel + swizzled(k, c + (odd ? 0 : 1))) = odd ? lo : hi;
+      }
+      ids = ids_of(j + 2);
+      fence_proxy_async_smem();
+      mbar_arrive(&full[st]);
+    }
+  } else {
+    // ------------------------------------------------------------------------------- the MMAs
+    reg_free<S::mma_regs>();
+    if (warp == kMma && lane == 0 && tiles > 0) {
+      const int slots = SLOTS == 2 && r0 + 128 < r1 ? 2 : 1;
+      constexpr uint32_t id_qk = idesc_f16(128, kKeys), id_pv = idesc_f16(128, D, 1);
+      const uint32_t q_at = smem_u32(q_img), k_at = smem_u32(k_img), v_at = smem_u32(v_img);
+      bool ok = true;
+      for (int s = 0; s < slots && ok; ++s) ok = mbar_wait(&bar.q_full[s], 0, err, kErrTimeoutFull);
+      auto qk = [&](int s, int buf, int j) {
+        const uint32_t kt = k_at + (j % S::stages) * S::stage;
+  #pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          const uint32_t off = (i >> 2) * kPanel + (i & 3) * 32;
+          mma_bf16(tmem + buf * 128, desc_kmajor_sw128(q_at + s * S::stage + off), desc_kmajor_sw128(kt + off), id_qk, i != 0);
+        }
+        mma_commit(&bar.s_full[buf]);
+        mbar_arrive(&bar.s_full[buf]);
+      };
+      auto pv = [&](int s, int buf, int j) {
+        const uint32_t vt = v_at + (j % S::stages) * S::stage;
+  #pragma unroll
+        for (int i = 0; i < kKeys / 16; ++i)
+          mma_f16_ts(tmem + S::o_col + s * D, tmem + buf * 128 + 8 * i, desc_mnmajor_sw128(vt + i * 2048, kPanel), id_pv,
+                     j > 0 || i != 0);
+      };
+      auto wait_k = [&](int j) { return mbar_wait(&bar.k_full[j % S::stages], (j / S::stages) & 1, err, kErrTimeoutFull); };
+      auto wait_v = [&](int j) { return mbar_wait(&bar.v_full[j % S::stages], (j / S::stages) & 1, err, kErrTimeoutFull); };
+      for (int j = 0; j <= tiles && ok; ++j) {
+        if constexpr (SLOTS == 2) {
+          for (int s = 0; s < slots && ok; ++s) {
+            if (j > 0) {
+              ok = wait_v(j - 1) && mbar_wait(&bar.p_full[s], (j - 1) & 1, err, kErrTimeoutFull);
+              if (!ok) break;
+              tc_fence_after();
+              pv(s, s, j - 1);
+              if (s == slots - 1) mma_commit(&bar.v_empty[(j - 1) % S::stages]);
+              if (j == tiles) mma_commit(&bar.o_full[s]);
+            }
+            if (j < tiles) {
+              ok = wait_k(j);
+              if (!ok) break;
+              tc_fence_after();
+              qk(s, s, j);
+              if (s == slots - 1) mma_commit(&bar.k_empty[j % S::stages]);
+            }
+          }
+        } else {
+          if (j < tiles) {
+            ok = wait_k(j);
+            if (!ok) break;
+            tc_fence_after();
+            qk(0, j & 1, j);
+            mma_commit(&bar.k_empty[j % S::stages]);
+          }
+          if (j > 0) {
+            ok = wait_v(j - 1) && mbar_wait(&bar.p_full[(j - 1) & 1], ((j - 1) >> 1) & 1, err, kErrTimeoutFull);
+            if (!ok) break;
+            tc_fence_after();
+            pv(0, (j - 1) & 1, j - 1);
+            mma_commit(&bar.v_empty[(j - 1) % S::stages]);
+            mma_commit(&bar.pv_done);
+            if (j == tiles) mma_commit(&bar.o_full[0]);
+          }
+        }
+      }
+      if (!ok) {  // a wait gave up: nothing of this thread's may run on when tensor memory is freed
+        mma_commit(&bar.drained);
+        mbar_wait(&bar.drained, 0, err, kErrTimeoutOther);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kMma) tmem_dealloc(tmem, 512);
+}
+
+template <int D, int SLOTS>
+cudaError_t prepare() {
+  using S = Shape<D, SLOTS>;
+  cudaError_t e = cudaFuncSetAttribute(kv8_prompt_kernel<D, SLOTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem);
+  if (e != cudaSuccess) return e;
+  cudaFuncAttributes at;
+  if ((e = cudaFuncGetAttributes(&at, kv8_prompt_kernel<D, SLOTS>)) != cudaSuccess) return e;
+  // the roles' registers come out of what the launch has: more than that would be waited for without end
+  if (at.numRegs != S::regs) return cudaErrorInvalidConfiguration;
+  return cudaSuccess;
+}
+
+template <int D, int SLOTS>
+cudaError_t run(const Kv8Attn& a) {
+  using S = Shape<D, SLOTS>;
+  const cudaError_t e = prepare<D, SLOTS>();
+  if (e != cudaSuccess) return e;
+  const dim3 grid(static_cast<unsigned>(a.pages.heads) * a.chunks, a.seqs.batch, a.row_groups);
+  kv8_prompt_kernel<D, SLOTS><<<grid, S::threads, S::smem, a.stream>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+}  // namespace kv8
+
+void kv8_prompt_plan(Kv8Attn& a, int sms) {
+  const long long rows = static_cast<long long>(a.seqs.tokens) * a.group;
+  a.tile_rows = a.head_dim == 256 || rows <= 128 ? 128 : 256;
+  a.row_groups = static_cast<int>((rows + a.tile_rows - 1) / a.tile_rows);
+  const long long tiles = static_cast<long long>(a.seqs.batch) * a.pages.heads * a.row_groups;
+  long long span = a.max_len;
+  if (a.window) span = std::min(span, static_cast<long long>(a.window) + a.tile_rows / a.group + 32);
+  span = std::max(span, 1ll);
+  // where the row groups do not fill the SMs, the keys are cut, into 512 at the least
+  const long long want = std::max(1ll, std::min(sms / tiles, span / 512));
+  const long long chunk = ((span + want - 1) / want + kv8::kKeys - 1) / kv8::kKeys * kv8::kKeys;
+  a.chunk = static_cast<int>(chunk);
+  a.chunks = static_cast<int>((span + chunk - 1) / chunk);
+}
+
+cudaError_t launch_kv8_prompt(const Kv8Attn& a) {
+  switch (a.head_dim * 1000 + a.tile_rows) {
+    case 64128: return kv8::run<64, 1>(a);
+    case 64256: return kv8::run<64, 2>(a);
+    case 128128: return kv8::run<128, 1>(a);
+    case 128256: return kv8::run<128, 2>(a);
+    case 256128: return kv8::run<256, 1>(a);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+cudaError_t kv8_read_error(int* code, cudaStream_t stream) {
+  void* at = nullptr;
+  cudaError_t e = cudaGetSymbolAddress(&at, kv8::g_error);
+  if (e == cudaSuccess) e = cudaMemcpyAsync(code, at, sizeof(int), cudaMemcpyDeviceToHost, stream);
+  if (e == cudaSuccess) e = cudaMemsetAsync(at, 0, sizeof(int), stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+  return e;
+}
+
+}  // namespace qhtp
