@@ -154,6 +154,92 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* e
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
 }
 
+// Where the two passes over a row's scores stand: its buffer, the tile's group constants, and the columns that the
+// row sees.  CAREFUL: the tile has columns that not every row sees, or a group whose scales are not plain.
+struct Tile {
+  uint32_t s_at;
+  const float4* scale;
+  float down;
+  int lo, hi;
+};
+
+// The largest exponent of the row in this tile, or `top` where that is larger.
+template <bool CAREFUL>
+__device__ __forceinline__ float row_max(const Tile& k, float top) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t x[32];
+    tmem_ld32(k.s_at + 32 * c, x);
+    tmem_ld_wait();
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const float4 sc = k.scale[2 * c + g];
+      if constexpr (CAREFUL) {
+        float best = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int col = 32 * c + 16 * g + e;
+          best = fmaxf(best, col < k.hi && col >= k.lo ? __uint_as_float(x[16 * g + e]) : -INFINITY);
+        }
+        if (best != -INFINITY) top = fmaxf(top, fmaf(best, sc.x * k.down, sc.y));
+      } else {
+        float best[2] = {__uint_as_float(x[16 * g]), __uint_as_float(x[16 * g + 1])};
+#pragma unroll
+        for (int e = 2; e < 14; e += 4) {
+          best[0] = max3(best[0], __uint_as_float(x[16 * g + e]), __uint_as_float(x[16 * g + e + 1]));
+          best[1] = max3(best[1], __uint_as_float(x[16 * g + e + 2]), __uint_as_float(x[16 * g + e + 3]));
+        }
+        best[0] = max3(best[0], __uint_as_float(x[16 * g + 14]), __uint_as_float(x[16 * g + 15]));
+        top = fmaxf(top, fmaf(fmaxf(best[0], best[1]), sc.x * k.down, sc.y));
+      }
+    }
+  }
+  return top;
+}
+
+// p over the columns of S that have been read, as f16; returns l with the row's sum added.
+template <bool CAREFUL>
+__device__ __forceinline__ float row_exp(const Tile& k, float base, float l) {
+  uint32_t x[2][32];
+  tmem_ld32(k.s_at, x[0]);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    tmem_ld_wait();
+    if (c < 3) tmem_ld32(k.s_at + 32 * (c + 1), x[(c + 1) & 1]);
+    uint32_t w[16];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const float4 sc = k.scale[2 * c + g];
+      const float f = sc.x * k.down, off = sc.y - base;
+      float2 sum[2];
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        float2 t = fma2(__uint_as_float(x[c & 1][16 * g + e]), __uint_as_float(x[c & 1][16 * g + e + 1]), f, off);
+        t.x = ex2(t.x), t.y = ex2(t.y);
+        if constexpr (CAREFUL) {
+          const int col = 32 * c + 16 * g + e;
+          t.x = col < k.hi && col >= k.lo ? t.x : 0.0f;
+          t.y = col + 1 < k.hi && col + 1 >= k.lo ? t.y : 0.0f;
+        }
+        sum[(e >> 1) & 1] = e < 4 ? t : add2(sum[(e >> 1) & 1], t);
+        w[8 * g + e / 2] = pack_half2(t.x, t.y);
+      }
+      sum[0] = add2(sum[0], sum[1]);
+      const float add = sum[0].x + sum[0].y;
+      if constexpr (CAREFUL) {
+        const bool zero = sc.z == kZeroTile;  // a tile of V whose scale counts as zero
+        if (add != 0.0f) l = fmaf(add, zero ? 0.5f * kZeroTile : sc.z, l);  // hidden keys add nothing, whatever their scale
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[8 * g + e] = zero ? 0u : w[8 * g + e];
+      } else {
+        l = fmaf(add, sc.z, l);
+      }
+    }
+    tmem_st16(k.s_at + 16 * c, w);
+  }
+  return l;
+}
+
 template <int D, int SLOTS>
 __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel(const Kv8Attn a) {
   using S = Shape<D, SLOTS>;
@@ -231,39 +317,12 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
       for (int j = 0; j < tiles; ++j) {
         const int buf = SLOTS == 2 ? slot : j & 1;
         const uint32_t phase = SLOTS == 2 ? j & 1 : (j >> 1) & 1;
-        const uint32_t s_at = lanes + buf * 128;
         if (!warp_wait(&bar.s_full[buf], phase, err, kErrTimeoutAccum)) break;
         tc_fence_after();
-        const float4* sc = s_scale[j & 3];
         const int key0 = keys.lo + j * kKeys;
-        const bool masked = key0 + kKeys > all_hi || key0 < all_lo;
-        const int hi = row_hi - key0, lo = row_lo - key0;  // visible columns [lo, hi)
-
-        // the row's maximum
-        float top = m;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t x[32];
-          tmem_ld32(s_at + 32 * c, x);
-          tmem_ld_wait();
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            float best = -INFINITY;
-            if (!masked) {
-#pragma unroll
-              for (int e = 0; e < 16; e += 2)
-                best = max3(best, __uint_as_float(x[16 * g + e]), __uint_as_float(x[16 * g + e + 1]));
-            } else {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const int col = 32 * c + 16 * g + e;
-                if (col < hi && col >= lo) best = fmaxf(best, __uint_as_float(x[16 * g + e]));
-              }
-            }
-            const float4 k = sc[2 * c + g];
-            if (best != -INFINITY) top = fmaxf(top, fmaf(best, k.x * down, k.y));
-          }
-        }
+        const Tile k{lanes + buf * 128, s_scale[j & 3], down, row_lo - key0, row_hi - key0};
+        const bool careful = key0 + kKeys > all_hi || key0 < all_lo || s_scale[j & 3][0].w != 0.0f;
+        const float top = careful ? row_max<true>(k, m) : row_max<false>(k, m);
         // raise m where it pays; rows of a warp move together
         if (__any_sync(0xffffffffu, top > m + kGrow || (m == -INFINITY && top != -INFINITY))) {
           const float alpha = m == -INFINITY ? 0.0f : ex2(m - top);
@@ -285,40 +344,7 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
           m = top;
         }
         const float base = m == -INFINITY ? 0.0f : m;
-        // p, its sum, and p as f16 over the columns of S that have been read
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t x[32], w[16];
-          tmem_ld32(s_at + 32 * c, x);
-          tmem_ld_wait();
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const float4 k = sc[2 * c + g];
-            const float f = k.x * down, off = k.y - base;
-            float2 sum = make_float2(0.0f, 0.0f);
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              float2 t = fma2(__uint_as_float(x[16 * g + e]), __uint_as_float(x[16 * g + e + 1]), f, off);
-              t.x = ex2(t.x), t.y = ex2(t.y);
-              if (masked) {
-                const int col = 32 * c + 16 * g + e;
-                t.x = col < hi && col >= lo ? t.x : 0.0f;
-                t.y = col + 1 < hi && col + 1 >= lo ? t.y : 0.0f;
-              }
-              sum = add2(sum, t);
-              w[8 * g + e / 2] = pack_half2(t.x, t.y);
-            }
-            const float add = sum.x + sum.y;
-            if (k.z == kZeroTile) {  // a tile of V whose scale counts as zero
-              l = fmaf(add, 0.5f * kZeroTile, l);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) w[8 * g + e] = 0;
-            } else if (!masked || add != 0.0f) {  // masked keys add nothing, whatever their scale is
-              l = fmaf(add, k.z, l);
-            }
-          }
-          tmem_st16(s_at + 16 * c, w);
-        }
+        l = careful ? row_exp<true>(k, base, l) : row_exp<false>(k, base, l);
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&bar.p_full[buf]);
@@ -407,7 +433,10 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
       const int st = j % S::stages;
       if (j >= S::stages && !warp_wait(&empty[st], ((j / S::stages) - 1) & 1, err, kErrTimeoutEmpty)) break;
       if (scales) {
-        if (lane < 8) s_scale[j & 3][lane] = make_float4(sc.c, sc.log2_w, sc.inv_w, 0.0f);
+        // .w: a group whose scales need care (zero, or not finite)
+        const bool odd = !(sc.inv_w < kZeroTile) || !isfinite(sc.c);
+        const float care = __any_sync(0xffffffffu, odd) ? 1.0f : 0.0f;
+        if (lane < 8) s_scale[j & 3][lane] = make_float4(sc.c, sc.log2_w, sc.inv_w, care);
         sc = block_scales(a, ids, h);
       }
       uint8_t* const to = img + st * S::stage;
