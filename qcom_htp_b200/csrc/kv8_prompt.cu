@@ -89,59 +89,50 @@ __device__ __forceinline__ uint32_t swizzled(int r, int c) {
   return static_cast<uint32_t>(r * 128 + (((c ^ r) & 7) << 4));
 }
 
-// The rows of one slot, scaled by a power of two each, as f16 into its image.
+// The rows of one slot as f16 into its image, rows of bf16 scaled by a power of two each.  D / 8 lanes a row, all of a
+// warp's rows in flight at once.
 template <int D>
 __device__ __forceinline__ void load_q(const Kv8Attn& a, int b, int h, long long row0, int r0, int r1, uint8_t* img,
                                        float* down_at, int warp, int lane) {
-  constexpr int E = D / 32;
-  constexpr int kBatch = 8;  // rows of a warp in flight
-  for (int base = 0; base < 32; base += kBatch) {
-    uint32_t w[kBatch][E / 2];
+  constexpr int kLanes = D / 8, kRows = 32 / kLanes;  // rows of a load
+  constexpr int kBatch = D == 256 ? 16 : 32 / kRows;  // loads in flight
+  const int sub = lane / kLanes, c = lane % kLanes;
+  const uint16_t* const q = static_cast<const uint16_t*>(a.q.data) + b * a.q.batch_stride + row0 * a.q.token_stride +
+                            static_cast<long long>(h) * a.group * a.q.head_stride + 8 * c;
+  // token and head of the lane's next row
+  int row = r0 + warp * 32 + sub;
+  int t = row / a.group, head = row - t * a.group;
+#pragma unroll 1
+  for (int base = 0; base < 32 / kRows; base += kBatch) {
+    uint4 w[kBatch];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      const int row = r0 + warp * 32 + base + i;
-#pragma unroll
-      for (int e = 0; e < E / 2; ++e) w[i][e] = 0;
-      if (row < r1) {
-        const int t = row / a.group;
-        const uint16_t* src = static_cast<const uint16_t*>(a.q.data) + b * a.q.batch_stride +
-                              (row0 + t) * a.q.token_stride +
-                              (static_cast<long long>(h) * a.group + row - t * a.group) * a.q.head_stride + lane * E;
-        if constexpr (E == 8) {
-          const uint4 v = __ldg(reinterpret_cast<const uint4*>(src));
-          w[i][0] = v.x, w[i][1] = v.y, w[i][2] = v.z, w[i][3] = v.w;
-        } else if constexpr (E == 4) {
-          const uint2 v = __ldg(reinterpret_cast<const uint2*>(src));
-          w[i][0] = v.x, w[i][1] = v.y;
-        } else {
-          w[i][0] = __ldg(reinterpret_cast<const uint32_t*>(src));
-        }
-      }
+      w[i] = make_uint4(0, 0, 0, 0);
+      if (row < r1) w[i] = __ldg(reinterpret_cast<const uint4*>(q + t * a.q.token_stride + head * a.q.head_stride));
+      row += kRows;
+      head += kRows;
+      while (head >= a.group) head -= a.group, ++t;
     }
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      const int r = warp * 32 + base + i;
-      float x[E];
+      const int r = warp * 32 + (base + i) * kRows + sub;
+      float down = 1.0f;
+      if (a.bf16) {
+        float x[8];
+        Vec<__nv_bfloat16>::load(w[i], x);
+        // bf16 magnitudes are ordered like their bits: the largest of the lane's, then of the row's
+        uint32_t top = __vmaxu2(__vmaxu2(w[i].x & 0x7fff7fffu, w[i].y & 0x7fff7fffu),
+                                __vmaxu2(w[i].z & 0x7fff7fffu, w[i].w & 0x7fff7fffu));
 #pragma unroll
-      for (int e = 0; e < E / 2; ++e) {
-        if (a.bf16) {
-          x[2 * e] = __uint_as_float(w[i][e] << 16), x[2 * e + 1] = __uint_as_float(w[i][e] & 0xffff0000u);
-        } else {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i][e]));
-          x[2 * e] = f.x, x[2 * e + 1] = f.y;
-        }
+        for (int o = 1; o < kLanes; o <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
+        top = max(top & 0xffffu, top >> 16);
+        float up;
+        row_factor(__uint_as_float(top << 16), up, down);
+        w[i] = make_uint4(pack_half2(x[0] * up, x[1] * up), pack_half2(x[2] * up, x[3] * up),
+                          pack_half2(x[4] * up, x[5] * up), pack_half2(x[6] * up, x[7] * up));
       }
-      uint32_t top = 0;
-#pragma unroll
-      for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-      top = __reduce_max_sync(0xffffffffu, top);
-      float up, down;
-      row_factor(__uint_as_float(top), up, down);
-      const int byte = lane * E * 2;
-      uint8_t* to = img + (byte >> 7) * kPanel + swizzled(r, (byte & 127) >> 4) + (byte & 15);
-#pragma unroll
-      for (int e = 0; e < E / 2; ++e) reinterpret_cast<uint32_t*>(to)[e] = pack_half2(x[2 * e] * up, x[2 * e + 1] * up);
-      if (lane == 0) down_at[r] = down;
+      *reinterpret_cast<uint4*>(img + (c >> 3) * kPanel + swizzled(r, c & 7)) = w[i];
+      if (c == 0) down_at[r] = down;
     }
   }
 }
@@ -248,7 +239,8 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
   __shared__ Barriers bar;
   __shared__ uint32_t s_tmem;
   __shared__ float s_down[SLOTS * 128];
-  __shared__ float4 s_scale[4][8];  // (c, log2 w, 1 / w) of a tile's 16-key groups, four tiles deep
+  __shared__ float4 s_scale[4][8];       // (c, log2 w, 1 / w, care) of a tile's 16-key groups, four tiles deep
+  __shared__ long long s_off[8][2][8];   // first code of a tile's 16-key groups, per converter warp, two tiles deep
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // heads fastest, the longest row groups (the last of a causal sequence) first
@@ -276,8 +268,8 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) {
         mbar_init(&bar.q_full[i], 128);
-        mbar_init(&bar.k_full[i], 128);
-        mbar_init(&bar.v_full[i], 128);
+        mbar_init(&bar.k_full[i], S::stages == 1 ? 256 : 128);
+        mbar_init(&bar.v_full[i], S::stages == 1 ? 256 : 128);
         mbar_init(&bar.k_empty[i], 1);
         mbar_init(&bar.v_empty[i], 1);
         mbar_init(&bar.s_full[i], 2);  // the MMAs, and the issuing thread's own arrival
@@ -398,69 +390,87 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
   } else if (warp < kMma) {
     // ------------------------------------------------------------------------------- codes to f16 images
     if constexpr (S::convert_regs < S::regs) reg_free<S::convert_regs>(); else reg_alloc<S::convert_regs>();
-    const bool is_v = warp >= kConvV;
+    // One warpgroup has K, the other V; where there is room for one tile of each only (head_dim 256), both take K and V in
+    // turn: each has to be rewritten while the other is multiplied.
+    constexpr bool kBoth = S::stages == 1;
+    constexpr int kThreads = kBoth ? 256 : 128, kStep = kThreads / (4 * S::panels), kPieces = 128 / kStep;
+    const bool is_v = !kBoth && warp >= kConvV;
     const int t = threadIdx.x - (is_v ? kConvV : kConvK) * 32;
-    constexpr int kPieces = D / 16;          // 16-code pieces of a key, and of a thread
-    const int8_t* const codes = is_v ? a.pages.v : a.pages.k;
-    uint64_t* const full = is_v ? bar.v_full : bar.k_full;
-    uint64_t* const empty = is_v ? bar.v_empty : bar.k_empty;
-    uint8_t* const img = is_v ? v_img : k_img;
-    const bool scales = warp == kConvK;      // this warp also brings the tiles' scales
+    // A thread has 16 codes of the keys row, row + kStep, ...; the eight threads of a 16-byte store have four pieces
+    // of two neighbouring rows of one panel, which the swizzle puts into eight different chunks.
+    const int row = ((t >> 3) / S::panels) * 2 + ((t >> 2) & 1), panel = (t >> 3) % S::panels, piece = t & 3;
+    const int from = (row & 15) * D + panel * 64 + piece * 16;  // in its 16-key group
+    const uint32_t to0 = panel * kPanel + swizzled(row, 2 * piece), to1 = panel * kPanel + swizzled(row, 2 * piece + 1);
+    const bool scales = warp == kConvK;  // this warp also brings the tiles' scales
     const int bs_log2 = a.pages.bs_log2, bs = 1 << bs_log2;
-    const int piece = t % kPieces;
+    long long(*const off)[8] = s_off[warp - kConvK];  // of two tiles' groups, each warp for itself
     // block of the tile's 16-key group `lane` (of eight); -1: none
     auto ids_of = [&](int j) {
       const int key = keys.lo + j * kKeys + 16 * (lane & 7);
       return j < tiles && key < keys.hi ? static_cast<int>(block_of(a.seqs, a.pages, b, key >> bs_log2)) : -1;
     };
-    auto load = [&](int j, int ids, int i) {
-      const int k = i * (128 / kPieces) + t / kPieces;  // key of the tile
-      const int id = max(__shfl_sync(0xffffffffu, ids, k >> 4), 0);
-      const int slot = (keys.lo + j * kKeys + k) & (bs - 1);
-      return __ldg(reinterpret_cast<const uint4*>(
-          codes + ((((static_cast<long long>(id) * a.pages.heads + h) << bs_log2) + slot) * D + 16 * piece)));
+    auto put_off = [&](int j, int id) {
+      const int slot = (keys.lo + j * kKeys + 16 * (lane & 7)) & (bs - 1);
+      if (lane < 8) off[j & 1][lane] = (((static_cast<long long>(max(id, 0)) * a.pages.heads + h) << bs_log2) + slot) * D;
+      __syncwarp();
     };
-    uint4 raw[kPieces];
-    int ids = ids_of(0);
-    if (tiles > 0) {
+    auto load = [&](const int8_t* codes, int j, int i) {
+      return __ldg(reinterpret_cast<const uint4*>(codes + off[j & 1][(i * kStep + row) >> 4] + from));
+    };
+    uint4 raw[kBoth ? 2 : 1][kPieces];
+    auto convert = [&](uint4(&x)[kPieces], const int8_t* codes, uint8_t* to, int next) {
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) raw[i] = load(0, ids, i);
+      for (int i = 0; i < kPieces; ++i) {
+        uint32_t u[8];
+        codes_to_half2(x[i].x, u[0], u[1]);
+        codes_to_half2(x[i].y, u[2], u[3]);
+        codes_to_half2(x[i].z, u[4], u[5]);
+        codes_to_half2(x[i].w, u[6], u[7]);
+        if (next < tiles) x[i] = load(codes, next, i);
+        *reinterpret_cast<uint4*>(to + to0 + i * kStep * 128) = make_uint4(u[0], u[1], u[2], u[3]);
+        *reinterpret_cast<uint4*>(to + to1 + i * kStep * 128) = make_uint4(u[4], u[5], u[6], u[7]);
+      }
+      fence_proxy_async_smem();
+    };
+    auto wait_empty = [&](uint64_t* empty, int j) {
+      return j < S::stages ||
+             warp_wait(&empty[j % S::stages], ((j / S::stages) - 1) & 1, err, kErrTimeoutEmpty);
+    };
+    const int8_t* const codes = is_v ? a.pages.v : a.pages.k;
+    int id = ids_of(0);
+    if (tiles > 0) {
+      put_off(0, id);
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        raw[0][i] = load(codes, 0, i);
+        if constexpr (kBoth) raw[1][i] = load(a.pages.v, 0, i);
+      }
     }
     BlockScales sc{};
-    if (scales && tiles > 0) sc = block_scales(a, ids, h);
-    ids = ids_of(1);
+    if (scales && tiles > 0) sc = block_scales(a, id, h);
+    id = ids_of(1);
     for (int j = 0; j < tiles; ++j) {
       const int st = j % S::stages;
-      if (j >= S::stages && !warp_wait(&empty[st], ((j / S::stages) - 1) & 1, err, kErrTimeoutEmpty)) break;
+      put_off(j + 1, id);
+      if (!wait_empty(is_v ? bar.v_empty : bar.k_empty, j)) break;
       if (scales) {
         // .w: a group whose scales need care (zero, or not finite)
         const bool odd = !(sc.inv_w < kZeroTile) || !isfinite(sc.c);
         const float care = __any_sync(0xffffffffu, odd) ? 1.0f : 0.0f;
         if (lane < 8) s_scale[j & 3][lane] = make_float4(sc.c, sc.log2_w, sc.inv_w, care);
-        sc = block_scales(a, ids, h);
+        sc = block_scales(a, id, h);
       }
-      uint8_t* const to = img + st * S::stage;
-#pragma unroll
-      for (int i = 0; i < kPieces; ++i) {
-        const uint4 x = raw[i];
-        if (j + 1 < tiles) raw[i] = load(j + 1, ids, i);
-        const int k = i * (128 / kPieces) + t / kPieces;
-        uint32_t u[8];
-        codes_to_half2(x.x, u[0], u[1]);
-        codes_to_half2(x.y, u[2], u[3]);
-        codes_to_half2(x.z, u[4], u[5]);
-        codes_to_half2(x.w, u[6], u[7]);
-        const uint4 lo = make_uint4(u[0], u[1], u[2], u[3]), hi = make_uint4(u[4], u[5], u[6], u[7]);
-        uint8_t* const panel = to + (piece >> 2) * kPanel;
-        const int c = 2 * (piece & 3);
-        // eight threads of a store fill eight different chunks: every other panel starts with the odd ones
-        const bool odd = (piece >> 2) & 1;
-        *reinterpret_cast<uint4*>(panel + swizzled(k, c + (odd ? 1 : 0))) = odd ? hi : lo;
-        *reinterpret_cast<uint4*>(panel + swizzled(k, c + (odd ? 0 : 1))) = odd ? lo : hi;
+      id = ids_of(j + 2);
+      if constexpr (kBoth) {
+        convert(raw[0], a.pages.k, k_img, j + 1);
+        mbar_arrive(&bar.k_full[0]);
+        if (!wait_empty(bar.v_empty, j)) break;
+        convert(raw[1], a.pages.v, v_img, j + 1);
+        mbar_arrive(&bar.v_full[0]);
+      } else {
+        convert(raw[0], codes, (is_v ? v_img : k_img) + st * S::stage, j + 1);
+        mbar_arrive(is_v ? &bar.v_full[st] : &bar.k_full[st]);
       }
-      ids = ids_of(j + 2);
-      fence_proxy_async_smem();
-      mbar_arrive(&full[st]);
     }
   } else {
     // ------------------------------------------------------------------------------- the MMAs
