@@ -26,6 +26,8 @@ namespace {
 
 constexpr int kKeys = 128;             // keys of a tile
 constexpr int kPanel = 128 * 128;      // bytes of a [128 rows][64 f16] swizzled image
+// pairs of a 16-key group whose exponentials are computed by polynomial, a bit each
+constexpr uint32_t kPoly = 0xAA;
 constexpr float kGrow = 8.0f;          // log2 of how far p may pass 1 before m follows
 
 template <int D, int SLOTS>
@@ -37,10 +39,10 @@ struct Shape {
   static constexpr int threads = (SLOTS + 3) * 128;
   // registers of a thread: at launch (the most that the threads leave room for), and by role; the roles' sum is the launch's
   static constexpr int regs = SLOTS == 2 ? 96 : 128;
-  static constexpr int softmax_regs = SLOTS == 2 ? 144 : 184;
-  static constexpr int convert_regs = SLOTS == 2 ? 72 : 136;
-  static constexpr int mma_regs = SLOTS == 2 ? 48 : 56;
-  static_assert(SLOTS * softmax_regs + 2 * convert_regs + mma_regs <= (SLOTS + 3) * regs, "registers");
+  static constexpr int softmax_regs = SLOTS == 2 ? 144 : 168;
+  static constexpr int convert_regs = SLOTS == 2 ? 72 : 128;
+  static constexpr int mma_regs = SLOTS == 2 ? 48 : 80;
+  static_assert(convert_regs <= regs && SLOTS * softmax_regs + 2 * convert_regs + mma_regs <= (SLOTS + 3) * regs, "registers");
   static constexpr int o_col = 256;                             // S buffers in columns 0..255
   static_assert(o_col + SLOTS * D <= 512, "tensor memory");
 };
@@ -83,6 +85,72 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "=f"(r.x), "=f"(r.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float c) {
+  float2 r;
+  asm("{\n\t.reg .b64 u, v, w, z;\n\t"
+      "mov.b64 u, {%2, %3};\n\tmov.b64 v, {%4, %5};\n\tmov.b64 w, {%6, %6};\n\t"
+      "fma.rn.f32x2 z, u, v, w;\n\t"
+      "mov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c));
+  return r;
+}
+// 2^t of a pair on the FMA pipe: t = n + f with n the nearest integer (it is left in the low bits of t + 1.5 2^23)
+// and |f| <= 1/2, 2^f by the degree-4 polynomial of least relative error there (2.6e-6, found by Remez exchange), n added
+// to the exponent.  t below -126 counts as -126.
+__device__ __forceinline__ float2 ex2_poly(float2 t) {
+  t.x = fmaxf(t.x, -126.0f), t.y = fmaxf(t.y, -126.0f);
+  const float2 big = add2(t, make_float2(12582912.0f, 12582912.0f));
+  const float2 n = add2(big, make_float2(-12582912.0f, -12582912.0f));
+  const float2 f = add2(t, make_float2(-n.x, -n.y));
+  float2 p = fma2(f.x, f.y, 0.009570102207362652f, 0.05591785907745361f);
+  p = fma2(p, f, 0.240247443318367f);
+  p = fma2(p, f, 0.6931217908859253f);
+  p = fma2(p, f, 0.9999992847442627f);
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(big.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(big.y) << 23)));
+}
+__device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ long long lds64(uint32_t at) {
+  long long r;
+  asm volatile("ld.shared.b64 %0, [%1];" : "=l"(r) : "r"(at) : "memory");
+  return r;
+}
+__device__ __forceinline__ float4 lds_f4(uint32_t at) {
+  float4 r;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(r.x), "=f"(r.y), "=f"(r.z), "=f"(r.w) : "r"(at) : "memory");
+  return r;
+}
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+// Low word of a descriptor of a 128-byte-swizzled image: start address and, for MN-major operands, the distance of
+// 64-element groups; the high word (1024 bytes between 8-row atoms, version 1, swizzle) is kDescHi.  Steps are added to
+// the low word in units of 16 bytes.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t at, uint32_t lbo) { return (at >> 4) | ((lbo >> 4) << 16); }
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(kDescHi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// A in tensor memory: one 32-bit column holds two consecutive K elements
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(kDescHi), "r"(idesc), "r"(accumulate)
+      : "memory");
 }
 // 16-byte chunk c of row r in a swizzled image
 __device__ __forceinline__ uint32_t swizzled(int r, int c) {
@@ -148,8 +216,7 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* e
 // Where the two passes over a row's scores stand: its buffer, the tile's group constants, and the columns that the
 // row sees.  CAREFUL: the tile has columns that not every row sees, or a group whose scales are not plain.
 struct Tile {
-  uint32_t s_at;
-  const float4* scale;
+  uint32_t s_at, scale;
   float down;
   int lo, hi;
 };
@@ -164,7 +231,7 @@ __device__ __forceinline__ float row_max(const Tile& k, float top) {
     tmem_ld_wait();
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
-      const float4 sc = k.scale[2 * c + g];
+      const float4 sc = lds_f4(k.scale + 16 * (2 * c + g));
       if constexpr (CAREFUL) {
         float best = -INFINITY;
 #pragma unroll
@@ -200,13 +267,16 @@ __device__ __forceinline__ float row_exp(const Tile& k, float base, float l) {
     uint32_t w[16];
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
-      const float4 sc = k.scale[2 * c + g];
+      const float4 sc = lds_f4(k.scale + 16 * (2 * c + g));
       const float f = sc.x * k.down, off = sc.y - base;
       float2 sum[2];
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
         float2 t = fma2(__uint_as_float(x[c & 1][16 * g + e]), __uint_as_float(x[c & 1][16 * g + e + 1]), f, off);
-        t.x = ex2(t.x), t.y = ex2(t.y);
+        if (!CAREFUL && kPoly >> (e / 2) & 1)
+          t = ex2_poly(t);
+        else
+          t.x = ex2(t.x), t.y = ex2(t.y);
         if constexpr (CAREFUL) {
           const int col = 32 * c + 16 * g + e;
           t.x = col < k.hi && col >= k.lo ? t.x : 0.0f;
@@ -312,7 +382,7 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
         if (!warp_wait(&bar.s_full[buf], phase, err, kErrTimeoutAccum)) break;
         tc_fence_after();
         const int key0 = keys.lo + j * kKeys;
-        const Tile k{lanes + buf * 128, s_scale[j & 3], down, row_lo - key0, row_hi - key0};
+        const Tile k{lanes + buf * 128, smem_u32(s_scale[j & 3]), down, row_lo - key0, row_hi - key0};
         const bool careful = key0 + kKeys > all_hi || key0 < all_lo || s_scale[j & 3][0].w != 0.0f;
         const float top = careful ? row_max<true>(k, m) : row_max<false>(k, m);
         // raise m where it pays; rows of a warp move together
@@ -389,7 +459,7 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
     }
   } else if (warp < kMma) {
     // ------------------------------------------------------------------------------- codes to f16 images
-    if constexpr (S::convert_regs < S::regs) reg_free<S::convert_regs>(); else reg_alloc<S::convert_regs>();
+    if constexpr (S::convert_regs < S::regs) reg_free<S::convert_regs>();
     // One warpgroup has K, the other V; where there is room for one tile of each only (head_dim 256), both take K and V in
     // turn: each has to be rewritten while the other is multiplied.
     constexpr bool kBoth = S::stages == 1;
@@ -403,7 +473,8 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
     const uint32_t to0 = panel * kPanel + swizzled(row, 2 * piece), to1 = panel * kPanel + swizzled(row, 2 * piece + 1);
     const bool scales = warp == kConvK;  // this warp also brings the tiles' scales
     const int bs_log2 = a.pages.bs_log2, bs = 1 << bs_log2;
-    long long(*const off)[8] = s_off[warp - kConvK];  // of two tiles' groups, each warp for itself
+    const uint32_t off = smem_u32(s_off[warp - kConvK]);  // of two tiles' groups, each warp for itself
+    const uint32_t off_row = off + (row >> 4) * 8;
     // block of the tile's 16-key group `lane` (of eight); -1: none
     auto ids_of = [&](int j) {
       const int key = keys.lo + j * kKeys + 16 * (lane & 7);
@@ -411,14 +482,16 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
     };
     auto put_off = [&](int j, int id) {
       const int slot = (keys.lo + j * kKeys + 16 * (lane & 7)) & (bs - 1);
-      if (lane < 8) off[j & 1][lane] = (((static_cast<long long>(max(id, 0)) * a.pages.heads + h) << bs_log2) + slot) * D;
+      if (lane < 8)
+        s_off[warp - kConvK][j & 1][lane] = (((static_cast<long long>(max(id, 0)) * a.pages.heads + h) << bs_log2) + slot) * D;
       __syncwarp();
     };
     auto load = [&](const int8_t* codes, int j, int i) {
-      return __ldg(reinterpret_cast<const uint4*>(codes + off[j & 1][(i * kStep + row) >> 4] + from));
+      // kStep is a multiple of 16
+      return __ldg(reinterpret_cast<const uint4*>(codes + lds64(off_row + (j & 1) * 64 + i * kStep / 16 * 8) + from));
     };
     uint4 raw[kBoth ? 2 : 1][kPieces];
-    auto convert = [&](uint4(&x)[kPieces], const int8_t* codes, uint8_t* to, int next) {
+    auto convert = [&](uint4(&x)[kPieces], const int8_t* codes, uint32_t to, int next) {
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
         uint32_t u[8];
@@ -427,8 +500,8 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
         codes_to_half2(x[i].z, u[4], u[5]);
         codes_to_half2(x[i].w, u[6], u[7]);
         if (next < tiles) x[i] = load(codes, next, i);
-        *reinterpret_cast<uint4*>(to + to0 + i * kStep * 128) = make_uint4(u[0], u[1], u[2], u[3]);
-        *reinterpret_cast<uint4*>(to + to1 + i * kStep * 128) = make_uint4(u[4], u[5], u[6], u[7]);
+        sts128(to + to0 + i * kStep * 128, u[0], u[1], u[2], u[3]);
+        sts128(to + to1 + i * kStep * 128, u[4], u[5], u[6], u[7]);
       }
       fence_proxy_async_smem();
     };
@@ -437,6 +510,7 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
              warp_wait(&empty[j % S::stages], ((j / S::stages) - 1) & 1, err, kErrTimeoutEmpty);
     };
     const int8_t* const codes = is_v ? a.pages.v : a.pages.k;
+    const uint32_t img = smem_u32(is_v ? v_img : k_img);
     int id = ids_of(0);
     if (tiles > 0) {
       put_off(0, id);
@@ -462,61 +536,72 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
       }
       id = ids_of(j + 2);
       if constexpr (kBoth) {
-        convert(raw[0], a.pages.k, k_img, j + 1);
+        convert(raw[0], a.pages.k, smem_u32(k_img), j + 1);
         mbar_arrive(&bar.k_full[0]);
         if (!wait_empty(bar.v_empty, j)) break;
-        convert(raw[1], a.pages.v, v_img, j + 1);
+        convert(raw[1], a.pages.v, smem_u32(v_img), j + 1);
         mbar_arrive(&bar.v_full[0]);
       } else {
-        convert(raw[0], codes, (is_v ? v_img : k_img) + st * S::stage, j + 1);
+        convert(raw[0], codes, img + st * S::stage, j + 1);
         mbar_arrive(is_v ? &bar.v_full[st] : &bar.k_full[st]);
       }
     }
   } else {
     // ------------------------------------------------------------------------------- the MMAs
     reg_free<S::mma_regs>();
-    if (warp == kMma && lane == 0 && tiles > 0) {
+    if (warp == kMma && tiles > 0) {
+      // The whole warp waits and one elected lane issues, so that addresses and descriptors stay in uniform registers:
+      // a lone thread's code moved each of them there per MMA, which took as long as the MMA itself.
       const int slots = SLOTS == 2 && r0 + 128 < r1 ? 2 : 1;
       constexpr uint32_t id_qk = idesc_f16(128, kKeys), id_pv = idesc_f16(128, D, 1);
-      const uint32_t q_at = smem_u32(q_img), k_at = smem_u32(k_img), v_at = smem_u32(v_img);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t q_desc = desc_lo(smem_u32(q_img), 16), k_desc = desc_lo(smem_u32(k_img), 16),
+                     v_desc = desc_lo(smem_u32(v_img), kPanel);
       bool ok = true;
-      for (int s = 0; s < slots && ok; ++s) ok = mbar_wait(&bar.q_full[s], 0, err, kErrTimeoutFull);
-      auto qk = [&](int s, int buf, int j) {
-        const uint32_t kt = k_at + (j % S::stages) * S::stage;
-  #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          const uint32_t off = (i >> 2) * kPanel + (i & 3) * 32;
-          mma_bf16(tmem + buf * 128, desc_kmajor_sw128(q_at + s * S::stage + off), desc_kmajor_sw128(kt + off), id_qk, i != 0);
+      for (int s = 0; s < slots && ok; ++s) ok = warp_wait(&bar.q_full[s], 0, err, kErrTimeoutFull);
+      auto qk = [&](int s, int buf, int j, bool last) {
+        const uint32_t kd = k_desc + (j % S::stages) * (S::stage >> 4), qd = q_desc + s * (S::stage >> 4);
+        if (elect_one()) {
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            constexpr uint32_t step = 32 >> 4, panel = kPanel >> 4;
+            const uint32_t off = (i >> 2) * panel + (i & 3) * step;
+            mma_ss(tm + buf * 128, qd + off, kd + off, id_qk, i != 0);
+          }
+          mma_commit(&bar.s_full[buf]);
+          mbar_arrive(&bar.s_full[buf]);
+          if (last) mma_commit(&bar.k_empty[j % S::stages]);
         }
-        mma_commit(&bar.s_full[buf]);
-        mbar_arrive(&bar.s_full[buf]);
+        __syncwarp();
       };
-      auto pv = [&](int s, int buf, int j) {
-        const uint32_t vt = v_at + (j % S::stages) * S::stage;
-  #pragma unroll
-        for (int i = 0; i < kKeys / 16; ++i)
-          mma_f16_ts(tmem + S::o_col + s * D, tmem + buf * 128 + 8 * i, desc_mnmajor_sw128(vt + i * 2048, kPanel), id_pv,
-                     j > 0 || i != 0);
+      auto pv = [&](int s, int buf, int j, bool last) {
+        const uint32_t vd = v_desc + (j % S::stages) * (S::stage >> 4);
+        if (elect_one()) {
+#pragma unroll
+          for (int i = 0; i < kKeys / 16; ++i)
+            mma_ts(tm + S::o_col + s * D, tm + buf * 128 + 8 * i, vd + i * (2048 >> 4), id_pv, j > 0 || i != 0);
+          if (last) mma_commit(&bar.v_empty[j % S::stages]);
+          if (SLOTS == 1) mma_commit(&bar.pv_done);
+          if (j == tiles - 1) mma_commit(&bar.o_full[s]);
+        }
+        __syncwarp();
       };
-      auto wait_k = [&](int j) { return mbar_wait(&bar.k_full[j % S::stages], (j / S::stages) & 1, err, kErrTimeoutFull); };
-      auto wait_v = [&](int j) { return mbar_wait(&bar.v_full[j % S::stages], (j / S::stages) & 1, err, kErrTimeoutFull); };
+      auto wait_k = [&](int j) { return warp_wait(&bar.k_full[j % S::stages], (j / S::stages) & 1, err, kErrTimeoutFull); };
+      auto wait_v = [&](int j) { return warp_wait(&bar.v_full[j % S::stages], (j / S::stages) & 1, err, kErrTimeoutFull); };
       for (int j = 0; j <= tiles && ok; ++j) {
         if constexpr (SLOTS == 2) {
           for (int s = 0; s < slots && ok; ++s) {
             if (j > 0) {
-              ok = wait_v(j - 1) && mbar_wait(&bar.p_full[s], (j - 1) & 1, err, kErrTimeoutFull);
+              ok = wait_v(j - 1) && warp_wait(&bar.p_full[s], (j - 1) & 1, err, kErrTimeoutFull);
               if (!ok) break;
               tc_fence_after();
-              pv(s, s, j - 1);
-              if (s == slots - 1) mma_commit(&bar.v_empty[(j - 1) % S::stages]);
-              if (j == tiles) mma_commit(&bar.o_full[s]);
+              pv(s, s, j - 1, s == slots - 1);
             }
             if (j < tiles) {
               ok = wait_k(j);
               if (!ok) break;
               tc_fence_after();
-              qk(s, s, j);
-              if (s == slots - 1) mma_commit(&bar.k_empty[j % S::stages]);
+              qk(s, s, j, s == slots - 1);
             }
           }
         } else {
@@ -524,23 +609,20 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
             ok = wait_k(j);
             if (!ok) break;
             tc_fence_after();
-            qk(0, j & 1, j);
-            mma_commit(&bar.k_empty[j % S::stages]);
+            qk(0, j & 1, j, true);
           }
           if (j > 0) {
-            ok = wait_v(j - 1) && mbar_wait(&bar.p_full[(j - 1) & 1], ((j - 1) >> 1) & 1, err, kErrTimeoutFull);
+            ok = wait_v(j - 1) && warp_wait(&bar.p_full[(j - 1) & 1], ((j - 1) >> 1) & 1, err, kErrTimeoutFull);
             if (!ok) break;
             tc_fence_after();
-            pv(0, (j - 1) & 1, j - 1);
-            mma_commit(&bar.v_empty[(j - 1) % S::stages]);
-            mma_commit(&bar.pv_done);
-            if (j == tiles) mma_commit(&bar.o_full[0]);
+            pv(0, (j - 1) & 1, j - 1, true);
           }
         }
       }
-      if (!ok) {  // a wait gave up: nothing of this thread's may run on when tensor memory is freed
-        mma_commit(&bar.drained);
-        mbar_wait(&bar.drained, 0, err, kErrTimeoutOther);
+      if (!ok) {  // a wait gave up: nothing issued here may run on when tensor memory is freed
+        if (elect_one()) mma_commit(&bar.drained);
+        __syncwarp();
+        warp_wait(&bar.drained, 0, err, kErrTimeoutOther);
       }
     }
   }
