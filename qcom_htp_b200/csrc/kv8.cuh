@@ -204,12 +204,17 @@ struct BlockScales {
   float c, log2_w, inv_w;
 };
 constexpr float kZeroTile = 36893488147419103232.0f;  // 2^65
-__device__ __forceinline__ BlockScales block_scales(const Kv8Attn& a, long long id, int h) {
-  if (id < 0) return {nan_f32(), nan_f32(), nan_f32()};
+struct RawScales {
+  float k, v;
+};
+__device__ __forceinline__ RawScales raw_scales(const Kv8Attn& a, long long id, int h) {
+  if (id < 0) return {nan_f32(), nan_f32()};
   const long long t = id * a.pages.heads + h;
-  const float w = a.pages.v_scale[t];
-  const float v = w < kScaleMin ? kScaleMin : w;  // a NaN stays
-  return {a.pages.k_scale[t] * a.scale_log2, log2f(v), w < kScaleMin ? kZeroTile : 1.0f / v};
+  return {a.pages.k_scale[t], a.pages.v_scale[t]};
+}
+__device__ __forceinline__ BlockScales fold_scales(const Kv8Attn& a, const RawScales& s) {
+  const float v = s.v < kScaleMin ? kScaleMin : s.v;  // a NaN stays
+  return {s.k * a.scale_log2, log2f(v), s.v < kScaleMin ? kZeroTile : 1.0f / v};
 }
 
 // 2^-e and the factor 2^e that brings a row of largest magnitude `top` to [2^14, 2^15): q then fits f16 without

@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_decode_kernel(const Kv8Attn a
     for (int i = threadIdx.x; i < nblk; i += kWarps * 32) {
       const long long id = block_of(a.seqs, a.pages, b, blk0 + i);
       s_off[i] = ((max(id, 0ll) * a.pages.heads + h) << bs_log2) * D;
-      const BlockScales s = block_scales(a, id, h);
+      const BlockScales s = fold_scales(a, raw_scales(a, id, h));
       s_c[i] = s.c, s_lw[i] = s.log2_w, s_iw[i] = s.inv_w;
     }
     __syncthreads();

@@ -35,7 +35,9 @@ struct Shape {
   static constexpr int panels = D / 64;
   static constexpr int stage = panels * kPanel;                 // a K or V tile
   static constexpr int stages = D == 256 ? 1 : 2;               // of K, and of V
-  static constexpr int smem = (SLOTS + 2 * stages) * stage + 1024;
+  static constexpr int staging = (D == 256 ? 1 : 2) * kKeys * D;  // codes on their way
+  static constexpr int smem = (SLOTS + 2 * stages) * stage + staging + 1024;
+  static_assert(smem + 2048 <= 227 * 1024, "shared memory");
   static constexpr int threads = (SLOTS + 3) * 128;
   // registers of a thread: at launch (the most that the threads leave room for), and by role; the roles' sum is the launch's
   static constexpr int regs = SLOTS == 2 ? 96 : 128;
@@ -48,7 +50,7 @@ struct Shape {
 };
 
 struct Barriers {
-  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done, o_full[2], drained;
+  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done, o_full[2], drained, staged[2];
 };
 
 template <int N>
@@ -114,10 +116,13 @@ __device__ __forceinline__ float2 ex2_poly(float2 t) {
 __device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-__device__ __forceinline__ long long lds64(uint32_t at) {
-  long long r;
-  asm volatile("ld.shared.b64 %0, [%1];" : "=l"(r) : "r"(at) : "memory");
+__device__ __forceinline__ uint2 lds64(uint32_t at) {
+  uint2 r;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(at) : "memory");
   return r;
+}
+__device__ __forceinline__ void named_barrier(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 __device__ __forceinline__ float4 lds_f4(uint32_t at) {
   float4 r;
@@ -310,7 +315,6 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
   __shared__ uint32_t s_tmem;
   __shared__ float s_down[SLOTS * 128];
   __shared__ float4 s_scale[4][8];       // (c, log2 w, 1 / w, care) of a tile's 16-key groups, four tiles deep
-  __shared__ long long s_off[8][2][8];   // first code of a tile's 16-key groups, per converter warp, two tiles deep
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // heads fastest, the longest row groups (the last of a causal sequence) first
@@ -331,6 +335,7 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
   uint8_t* const q_img = smem;
   uint8_t* const k_img = smem + SLOTS * S::stage;
   uint8_t* const v_img = k_img + S::stages * S::stage;
+  uint8_t* const stage_img = v_img + S::stages * S::stage;
 
   constexpr int kConvK = SLOTS * 4, kConvV = kConvK + 4, kMma = kConvV + 4;  // first warps of the roles
   if (warp == kMma) {
@@ -348,6 +353,8 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
       }
       mbar_init(&bar.pv_done, 1);
       mbar_init(&bar.drained, 1);
+      mbar_init(&bar.staged[0], 1);
+      mbar_init(&bar.staged[1], 1);
       fence_barrier_init();
     }
     tmem_relinquish();
@@ -461,47 +468,55 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
     // ------------------------------------------------------------------------------- codes to f16 images
     if constexpr (S::convert_regs < S::regs) reg_free<S::convert_regs>();
     // One warpgroup has K, the other V; where there is room for one tile of each only (head_dim 256), both take K and V in
-    // turn: each has to be rewritten while the other is multiplied.
+    // turn: each has to be rewritten while the other is multiplied.  The codes come by bulk copies into a staging tile
+    // (a 16-key group of a head is contiguous in its block), the next one as soon as this one is in registers.
     constexpr bool kBoth = S::stages == 1;
-    constexpr int kThreads = kBoth ? 256 : 128, kStep = kThreads / (4 * S::panels), kPieces = 128 / kStep;
+    constexpr int kThreads = kBoth ? 256 : 128, kStep = kThreads / (D / 8), kSteps = kKeys / kStep;
     const bool is_v = !kBoth && warp >= kConvV;
     const int t = threadIdx.x - (is_v ? kConvV : kConvK) * 32;
-    // A thread has 16 codes of the keys row, row + kStep, ...; the eight threads of a 16-byte store have four pieces
-    // of two neighbouring rows of one panel, which the swizzle puts into eight different chunks.
-    const int row = ((t >> 3) / S::panels) * 2 + ((t >> 2) & 1), panel = (t >> 3) % S::panels, piece = t & 3;
-    const int from = (row & 15) * D + panel * 64 + piece * 16;  // in its 16-key group
-    const uint32_t to0 = panel * kPanel + swizzled(row, 2 * piece), to1 = panel * kPanel + swizzled(row, 2 * piece + 1);
-    const bool scales = warp == kConvK;  // this warp also brings the tiles' scales
+    // A thread has chunk c (eight codes, 16 bytes as f16) of the rows row, row + kStep, ...: loads and stores of a
+    // warp are whole rows, without bank conflicts, and the swizzle of its rows is one number (kStep is a multiple of 8).
+    static_assert(kStep % 8 == 0, "swizzle");
+    const int c = t % (D / 8), row = t / (D / 8);
+    const uint32_t from = smem_u32(stage_img) + (is_v ? kKeys * D : 0) + row * D + c * 8;
+    const uint32_t to = (c >> 3) * kPanel + swizzled(row, c & 7);
+    const bool copies = kBoth ? warp == kConvK : (warp & 3) == 0, scales = warp == kConvK;
     const int bs_log2 = a.pages.bs_log2, bs = 1 << bs_log2;
-    const uint32_t off = smem_u32(s_off[warp - kConvK]);  // of two tiles' groups, each warp for itself
-    const uint32_t off_row = off + (row >> 4) * 8;
+    uint64_t* const staged = &bar.staged[is_v ? 1 : 0];
     // block of the tile's 16-key group `lane` (of eight); -1: none
     auto ids_of = [&](int j) {
       const int key = keys.lo + j * kKeys + 16 * (lane & 7);
       return j < tiles && key < keys.hi ? static_cast<int>(block_of(a.seqs, a.pages, b, key >> bs_log2)) : -1;
     };
-    auto put_off = [&](int j, int id) {
-      const int slot = (keys.lo + j * kKeys + 16 * (lane & 7)) & (bs - 1);
-      if (lane < 8)
-        s_off[warp - kConvK][j & 1][lane] = (((static_cast<long long>(max(id, 0)) * a.pages.heads + h) << bs_log2) + slot) * D;
+    // groups that there are none of keep the codes that happen to be there: they are hidden, or their scales are NaN
+    int issued = 0;
+    auto copy = [&](const int8_t* codes, int j, int id) {
+      ++issued;
+      const bool there = lane < 8 && id >= 0;
+      const int n = __popc(__ballot_sync(0xffffffffu, there));
+      if (lane == 0) mbar_arrive_expect_tx(staged, n * 16 * D);
       __syncwarp();
+      if (there) {
+        const int slot = (keys.lo + j * kKeys + 16 * lane) & (bs - 1);
+        bulk_load(stage_img + (is_v ? kKeys * D : 0) + lane * 16 * D,
+                  codes + (((static_cast<long long>(id) * a.pages.heads + h) << bs_log2) + slot) * D, 16 * D, staged);
+      }
     };
-    auto load = [&](const int8_t* codes, int j, int i) {
-      // kStep is a multiple of 16
-      return __ldg(reinterpret_cast<const uint4*>(codes + lds64(off_row + (j & 1) * 64 + i * kStep / 16 * 8) + from));
-    };
-    uint4 raw[kBoth ? 2 : 1][kPieces];
-    auto convert = [&](uint4(&x)[kPieces], const int8_t* codes, uint32_t to, int next) {
+    uint2 raw[kSteps];
+    auto fetch = [&](uint32_t phase) {
+      if (!warp_wait(staged, phase, err, kErrTimeoutFull)) return false;
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) {
-        uint32_t u[8];
-        codes_to_half2(x[i].x, u[0], u[1]);
-        codes_to_half2(x[i].y, u[2], u[3]);
-        codes_to_half2(x[i].z, u[4], u[5]);
-        codes_to_half2(x[i].w, u[6], u[7]);
-        if (next < tiles) x[i] = load(codes, next, i);
-        sts128(to + to0 + i * kStep * 128, u[0], u[1], u[2], u[3]);
-        sts128(to + to1 + i * kStep * 128, u[4], u[5], u[6], u[7]);
+      for (int i = 0; i < kSteps; ++i) raw[i] = lds64(from + i * kStep * D);
+      named_barrier(is_v ? 2 : 1, kThreads);  // the staging tile is read
+      return true;
+    };
+    auto convert = [&](uint32_t img) {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        uint32_t u[4];
+        codes_to_half2(raw[i].x, u[0], u[1]);
+        codes_to_half2(raw[i].y, u[2], u[3]);
+        sts128(img + to + i * kStep * 128, u[0], u[1], u[2], u[3]);
       }
       fence_proxy_async_smem();
     };
@@ -511,41 +526,51 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
     };
     const int8_t* const codes = is_v ? a.pages.v : a.pages.k;
     const uint32_t img = smem_u32(is_v ? v_img : k_img);
-    int id = ids_of(0);
+    int id = ids_of(0), id_next = ids_of(1);
+    RawScales sc{}, sc_next{};
     if (tiles > 0) {
-      put_off(0, id);
-#pragma unroll
-      for (int i = 0; i < kPieces; ++i) {
-        raw[0][i] = load(codes, 0, i);
-        if constexpr (kBoth) raw[1][i] = load(a.pages.v, 0, i);
-      }
+      if (copies) copy(codes, 0, id);
+      if (scales) sc = raw_scales(a, id, h);
     }
-    BlockScales sc{};
-    if (scales && tiles > 0) sc = block_scales(a, id, h);
-    id = ids_of(1);
-    for (int j = 0; j < tiles; ++j) {
+    bool ok = true;
+    for (int j = 0; j < tiles && ok; ++j) {
       const int st = j % S::stages;
-      put_off(j + 1, id);
-      if (!wait_empty(is_v ? bar.v_empty : bar.k_empty, j)) break;
+      const int id_after = ids_of(j + 2);
+      if (scales) sc_next = raw_scales(a, id_next, h);
+      if constexpr (kBoth) {
+        ok = fetch(0);
+        if (ok && copies) copy(a.pages.v, j, id);
+        ok = ok && wait_empty(bar.k_empty, j);
+      } else {
+        ok = fetch(j & 1);
+        if (ok && copies && j + 1 < tiles) copy(codes, j + 1, id_next);
+        ok = ok && wait_empty(is_v ? bar.v_empty : bar.k_empty, j);
+      }
+      if (!ok) break;
       if (scales) {
         // .w: a group whose scales need care (zero, or not finite)
-        const bool odd = !(sc.inv_w < kZeroTile) || !isfinite(sc.c);
+        const BlockScales f = fold_scales(a, sc);
+        const bool odd = !(f.inv_w < kZeroTile) || !isfinite(f.c);
         const float care = __any_sync(0xffffffffu, odd) ? 1.0f : 0.0f;
-        if (lane < 8) s_scale[j & 3][lane] = make_float4(sc.c, sc.log2_w, sc.inv_w, care);
-        sc = block_scales(a, id, h);
+        if (lane < 8) s_scale[j & 3][lane] = make_float4(f.c, f.log2_w, f.inv_w, care);
       }
-      id = ids_of(j + 2);
       if constexpr (kBoth) {
-        convert(raw[0], a.pages.k, smem_u32(k_img), j + 1);
+        convert(img);
         mbar_arrive(&bar.k_full[0]);
-        if (!wait_empty(bar.v_empty, j)) break;
-        convert(raw[1], a.pages.v, smem_u32(v_img), j + 1);
+        ok = fetch(1);
+        if (ok && copies && j + 1 < tiles) copy(a.pages.k, j + 1, id_next);
+        ok = ok && wait_empty(bar.v_empty, j);
+        if (!ok) break;
+        convert(smem_u32(v_img));
         mbar_arrive(&bar.v_full[0]);
       } else {
-        convert(raw[0], codes, img + st * S::stage, j + 1);
+        convert(img + st * S::stage);
         mbar_arrive(is_v ? &bar.v_full[st] : &bar.k_full[st]);
       }
+      id = id_next, id_next = id_after, sc = sc_next;
     }
+    // a wait gave up: copies under way end before the block does
+    if (!ok && copies) warp_wait(staged, (issued - 1) & 1, err, kErrTimeoutOther);
   } else {
     // ------------------------------------------------------------------------------- the MMAs
     reg_free<S::mma_regs>();
