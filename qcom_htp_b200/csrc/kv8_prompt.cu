@@ -4,15 +4,15 @@
 // sum 2^(t - m) cv / sum 2^(t - m) / sv, the int8 codes as f16 operands, V's scale in the exponent.
 //
 // A CTA owns SLOTS tiles of 128 query rows (the tokens and heads of one kv head's group, packed) and walks
-// over the keys 128 at a time:
-//   K and V converters (a warpgroup each) load codes from the paged cache to registers, one tile ahead, and
-//     write them as f16 into 128-byte-swizzled images [key][64 head_dim]: K-major for Q K^T, and the same
-//     bytes MN-major for P V;
-//   one thread issues the MMAs: S = Q K^T into tensor memory, O += P V with P read from tensor memory;
+// over the keys 64 at a time:
+//   K and V converters (a warpgroup each) bring codes from the paged cache by bulk copies into a staging tile (a 16-key
+//     group of a head is contiguous in its block) and write them as f16 into 128-byte-swizzled images
+//     [key][64 head_dim], three or four units ahead: K-major for Q K^T, and the same bytes MN-major for P V;
+//   one warp issues the MMAs: S = Q K^T into tensor memory, O += P V with P read from tensor memory;
 //   a softmax warpgroup per slot, a thread per row: S from tensor memory, P back over it as f16.
-// SLOTS = 2: the two tiles take turns, one's softmax under the other's MMAs.  SLOTS = 1 (one tile's rows, or
-// head_dim 256, whose O fills tensor memory): two S buffers, the softmax of one key tile under the MMAs of
-// its neighbours.
+// Each slot has two S buffers, so that the softmax of one unit runs under the MMAs of its neighbours and of the other
+// slot.  Q stands in tensor memory where that has room beside S and O (all but two slots of head_dim 128): an MMA then
+// reads 2 KB of shared memory where it reads 6, and those are what its rate hangs on at 64 keys.
 //
 // m is raised, and O rescaled, only when a row's maximum has grown by more than 2^8: p then stays below
 // 2^8, far inside f16, and most tiles leave O alone.
@@ -24,33 +24,41 @@ namespace qhtp {
 namespace kv8 {
 namespace {
 
-constexpr int kKeys = 128;             // keys of a tile
-constexpr int kPanel = 128 * 128;      // bytes of a [128 rows][64 f16] swizzled image
+constexpr int kKeys = 64;              // keys of a unit
+constexpr int kPanel = kKeys * 128;    // bytes of a [64 keys][64 f16] swizzled image
+constexpr int kQPanel = 128 * 128;     // and of a [128 rows][64 f16] one
 // pairs of a 16-key group whose exponentials are computed by polynomial, a bit each
-constexpr uint32_t kPoly = 0xAA;
+constexpr uint32_t kPoly = 0x00;
 constexpr float kGrow = 8.0f;          // log2 of how far p may pass 1 before m follows
 
 template <int D, int SLOTS>
 struct Shape {
   static constexpr int panels = D / 64;
-  static constexpr int stage = panels * kPanel;                 // a K or V tile
-  static constexpr int stages = D == 256 ? 1 : 2;               // of K, and of V
-  static constexpr int staging = (D == 256 ? 1 : 2) * kKeys * D;  // codes on their way
-  static constexpr int smem = (SLOTS + 2 * stages) * stage + staging + 1024;
+  static constexpr int unit = panels * kPanel;                  // 64 keys of K or V
+  static constexpr int units = D == 256 ? 3 : 4;                // of K, and of V
+  static constexpr int q_tile = panels * kQPanel;
+  // Q's image: where tensor memory takes Q and there is no room for both, it passes through V's last units
+  static constexpr int q_smem = D == 256 ? 0 : SLOTS * q_tile;
+  static constexpr int staging = 2 * kKeys * D;                 // codes on their way
+  static constexpr int smem = q_smem + 2 * units * unit + staging + 1024;
   static_assert(smem + 2048 <= 227 * 1024, "shared memory");
   static constexpr int threads = (SLOTS + 3) * 128;
   // registers of a thread: at launch (the most that the threads leave room for), and by role; the roles' sum is the launch's
   static constexpr int regs = SLOTS == 2 ? 96 : 128;
-  static constexpr int softmax_regs = SLOTS == 2 ? 144 : 168;
-  static constexpr int convert_regs = SLOTS == 2 ? 72 : 128;
+  static constexpr int softmax_regs = SLOTS == 2 ? 144 : 184;
+  static constexpr int convert_regs = SLOTS == 2 ? 72 : 120;
   static constexpr int mma_regs = SLOTS == 2 ? 48 : 80;
   static_assert(convert_regs <= regs && SLOTS * softmax_regs + 2 * convert_regs + mma_regs <= (SLOTS + 3) * regs, "registers");
-  static constexpr int o_col = 256;                             // S buffers in columns 0..255
-  static_assert(o_col + SLOTS * D <= 512, "tensor memory");
+  // tensor memory columns: S buffers from 0 (64 each, two per slot), O, Q
+  static constexpr bool q_tmem = SLOTS == 1 || D == 64;
+  static constexpr int q_col = SLOTS == 1 ? 128 : 384;
+  static constexpr int o_col = 256;
+  static_assert(o_col + SLOTS * D <= 512 && (!q_tmem || (SLOTS == 1 ? q_col + D / 2 <= o_col : o_col + SLOTS * D <= q_col)),
+                "tensor memory");
 };
 
 struct Barriers {
-  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done, o_full[2], drained, staged[2];
+  uint64_t q_full[2], k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[4], p_full[4], pv_done[2], drained, staged[2];
 };
 
 template <int N>
@@ -124,38 +132,47 @@ __device__ __forceinline__ uint2 lds64(uint32_t at) {
 __device__ __forceinline__ void named_barrier(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
-__device__ __forceinline__ float4 lds_f4(uint32_t at) {
-  float4 r;
-  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(r.x), "=f"(r.y), "=f"(r.z), "=f"(r.w) : "r"(at) : "memory");
-  return r;
-}
 // One lane of a converged warp.
-__device__ __forceinline__ bool elect_one() {
+__device__ __forceinline__ uint32_t elect_one() {
   uint32_t r;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
-  return r != 0;
+  return r;
 }
 // Low word of a descriptor of a 128-byte-swizzled image: start address and, for MN-major operands, the distance of
 // 64-element groups; the high word (1024 bytes between 8-row atoms, version 1, swizzle) is kDescHi.  Steps are added to
 // the low word in units of 16 bytes.
 constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
 __device__ __forceinline__ uint32_t desc_lo(uint32_t at, uint32_t lbo) { return (at >> 4) | ((lbo >> 4) << 16); }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+// The MMAs and commits are predicated on `leader`, not branched around: the code stays converged, and the compiler keeps
+// addresses and descriptors in uniform registers.
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
-      "setp.ne.b32 p, %5, 0;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
-      "r"(a_lo), "r"(b_lo), "r"(kDescHi), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(kDescHi), "r"(idesc), "r"(accumulate), "r"(leader)
       : "memory");
 }
 // A in tensor memory: one 32-bit column holds two consecutive K elements
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
-      "setp.ne.b32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
-      "r"(a), "r"(b_lo), "r"(kDescHi), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\tmov.b64 b, {%2, %3};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(kDescHi), "r"(idesc), "r"(accumulate), "r"(leader)
       : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t leader, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+      "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void arrive(uint32_t leader, uint32_t bar) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(bar),
+               "r"(leader)
+               : "memory");
 }
 // 16-byte chunk c of row r in a swizzled image
 __device__ __forceinline__ uint32_t swizzled(int r, int c) {
@@ -204,7 +221,7 @@ __device__ __forceinline__ void load_q(const Kv8Attn& a, int b, int h, long long
         w[i] = make_uint4(pack_half2(x[0] * up, x[1] * up), pack_half2(x[2] * up, x[3] * up),
                           pack_half2(x[4] * up, x[5] * up), pack_half2(x[6] * up, x[7] * up));
       }
-      *reinterpret_cast<uint4*>(img + (c >> 3) * kPanel + swizzled(r, c & 7)) = w[i];
+      *reinterpret_cast<uint4*>(img + (c >> 3) * kQPanel + swizzled(r, c & 7)) = w[i];
       if (c == 0) down_at[r] = down;
     }
   }
@@ -218,90 +235,78 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* e
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
 }
 
-// Where the two passes over a row's scores stand: its buffer, the tile's group constants, and the columns that the
-// row sees.  CAREFUL: the tile has columns that not every row sees, or a group whose scales are not plain.
-struct Tile {
-  uint32_t s_at, scale;
+// A row's view of a unit: the group constants, and the columns that the row sees.  CAREFUL below: the unit has columns
+// that not every row sees, or a group whose scales are not plain.
+struct View {
+  const float4* scale;
   float down;
   int lo, hi;
 };
 
-// The largest exponent of the row in this tile, or `top` where that is larger.
+// The largest exponent of the row in this unit, or `top` where that is larger.
 template <bool CAREFUL>
-__device__ __forceinline__ float row_max(const Tile& k, float top) {
+__device__ __forceinline__ float row_max(const View& k, const uint32_t (&x)[2][32], float top) {
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    uint32_t x[32];
-    tmem_ld32(k.s_at + 32 * c, x);
-    tmem_ld_wait();
+    const float4 sc = k.scale[c];
+    const uint32_t* const v = &x[c >> 1][16 * (c & 1)];
+    if constexpr (CAREFUL) {
+      float best = -INFINITY;
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      const float4 sc = lds_f4(k.scale + 16 * (2 * c + g));
-      if constexpr (CAREFUL) {
-        float best = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int col = 32 * c + 16 * g + e;
-          best = fmaxf(best, col < k.hi && col >= k.lo ? __uint_as_float(x[16 * g + e]) : -INFINITY);
-        }
-        if (best != -INFINITY) top = fmaxf(top, fmaf(best, sc.x * k.down, sc.y));
-      } else {
-        float best[2] = {__uint_as_float(x[16 * g]), __uint_as_float(x[16 * g + 1])};
-#pragma unroll
-        for (int e = 2; e < 14; e += 4) {
-          best[0] = max3(best[0], __uint_as_float(x[16 * g + e]), __uint_as_float(x[16 * g + e + 1]));
-          best[1] = max3(best[1], __uint_as_float(x[16 * g + e + 2]), __uint_as_float(x[16 * g + e + 3]));
-        }
-        best[0] = max3(best[0], __uint_as_float(x[16 * g + 14]), __uint_as_float(x[16 * g + 15]));
-        top = fmaxf(top, fmaf(fmaxf(best[0], best[1]), sc.x * k.down, sc.y));
+      for (int e = 0; e < 16; ++e) {
+        const int col = 16 * c + e;
+        best = fmaxf(best, col < k.hi && col >= k.lo ? __uint_as_float(v[e]) : -INFINITY);
       }
+      if (best != -INFINITY) top = fmaxf(top, fmaf(best, sc.x * k.down, sc.y));
+    } else {
+      float best[2] = {__uint_as_float(v[0]), __uint_as_float(v[1])};
+#pragma unroll
+      for (int e = 2; e < 14; e += 4) {
+        best[0] = max3(best[0], __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+        best[1] = max3(best[1], __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
+      }
+      best[0] = max3(best[0], __uint_as_float(v[14]), __uint_as_float(v[15]));
+      top = fmaxf(top, fmaf(fmaxf(best[0], best[1]), sc.x * k.down, sc.y));
     }
   }
   return top;
 }
 
-// p over the columns of S that have been read, as f16; returns l with the row's sum added.
+// p as f16 pairs into w; returns l with the row's sum added.
 template <bool CAREFUL>
-__device__ __forceinline__ float row_exp(const Tile& k, float base, float l) {
-  uint32_t x[2][32];
-  tmem_ld32(k.s_at, x[0]);
+__device__ __forceinline__ float row_exp(const View& k, const uint32_t (&x)[2][32], float base, float l, uint32_t (&w)[2][16]) {
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    tmem_ld_wait();
-    if (c < 3) tmem_ld32(k.s_at + 32 * (c + 1), x[(c + 1) & 1]);
-    uint32_t w[16];
+    const float4 sc = k.scale[c];
+    const uint32_t* const v = &x[c >> 1][16 * (c & 1)];
+    uint32_t* const to = &w[c >> 1][8 * (c & 1)];
+    const float f = sc.x * k.down, off = sc.y - base;
+    float2 sum[2];
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      const float4 sc = lds_f4(k.scale + 16 * (2 * c + g));
-      const float f = sc.x * k.down, off = sc.y - base;
-      float2 sum[2];
-#pragma unroll
-      for (int e = 0; e < 16; e += 2) {
-        float2 t = fma2(__uint_as_float(x[c & 1][16 * g + e]), __uint_as_float(x[c & 1][16 * g + e + 1]), f, off);
-        if (!CAREFUL && kPoly >> (e / 2) & 1)
-          t = ex2_poly(t);
-        else
-          t.x = ex2(t.x), t.y = ex2(t.y);
-        if constexpr (CAREFUL) {
-          const int col = 32 * c + 16 * g + e;
-          t.x = col < k.hi && col >= k.lo ? t.x : 0.0f;
-          t.y = col + 1 < k.hi && col + 1 >= k.lo ? t.y : 0.0f;
-        }
-        sum[(e >> 1) & 1] = e < 4 ? t : add2(sum[(e >> 1) & 1], t);
-        w[8 * g + e / 2] = pack_half2(t.x, t.y);
-      }
-      sum[0] = add2(sum[0], sum[1]);
-      const float add = sum[0].x + sum[0].y;
+    for (int e = 0; e < 16; e += 2) {
+      float2 t = fma2(__uint_as_float(v[e]), __uint_as_float(v[e + 1]), f, off);
+      if (!CAREFUL && kPoly >> (e / 2) & 1)
+        t = ex2_poly(t);
+      else
+        t.x = ex2(t.x), t.y = ex2(t.y);
       if constexpr (CAREFUL) {
-        const bool zero = sc.z == kZeroTile;  // a tile of V whose scale counts as zero
-        if (add != 0.0f) l = fmaf(add, zero ? 0.5f * kZeroTile : sc.z, l);  // hidden keys add nothing, whatever their scale
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[8 * g + e] = zero ? 0u : w[8 * g + e];
-      } else {
-        l = fmaf(add, sc.z, l);
+        const int col = 16 * c + e;
+        t.x = col < k.hi && col >= k.lo ? t.x : 0.0f;
+        t.y = col + 1 < k.hi && col + 1 >= k.lo ? t.y : 0.0f;
       }
+      sum[(e >> 1) & 1] = e < 4 ? t : add2(sum[(e >> 1) & 1], t);
+      to[e / 2] = pack_half2(t.x, t.y);
     }
-    tmem_st16(k.s_at + 16 * c, w);
+    sum[0] = add2(sum[0], sum[1]);
+    const float add = sum[0].x + sum[0].y;
+    if constexpr (CAREFUL) {
+      const bool zero = sc.z == kZeroTile;  // a tile of V whose scale counts as zero
+      if (add != 0.0f) l = fmaf(add, zero ? 0.5f * kZeroTile : sc.z, l);  // hidden keys add nothing, whatever their scale
+#pragma unroll
+      for (int e = 0; e < 8; ++e) to[e] = zero ? 0u : to[e];
+    } else {
+      l = fmaf(add, sc.z, l);
+    }
   }
   return l;
 }
@@ -314,7 +319,7 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
   __shared__ Barriers bar;
   __shared__ uint32_t s_tmem;
   __shared__ float s_down[SLOTS * 128];
-  __shared__ float4 s_scale[4][8];       // (c, log2 w, 1 / w, care) of a tile's 16-key groups, four tiles deep
+  __shared__ float4 s_scale[8][4];       // (c, log2 w, 1 / w, care) of a unit's 16-key groups, eight units deep
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // heads fastest, the longest row groups (the last of a causal sequence) first
@@ -328,33 +333,34 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
   const int len = seq_length(a, b);
   const Span all = row_span(a, len, T, r0, r1);
   const Span keys = chunk_span(a, all, chunk);
-  const int tiles = keys.lo < keys.hi ? (keys.hi - keys.lo + kKeys - 1) / kKeys : 0;
-  if (tiles == 0 && chunk > 0) return;
+  const int units = keys.lo < keys.hi ? (keys.hi - keys.lo + kKeys - 1) / kKeys : 0;
+  if (units == 0 && chunk > 0) return;
 
   uint8_t* const smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  uint8_t* const q_img = smem;
-  uint8_t* const k_img = smem + SLOTS * S::stage;
-  uint8_t* const v_img = k_img + S::stages * S::stage;
-  uint8_t* const stage_img = v_img + S::stages * S::stage;
+  uint8_t* const k_img = smem + S::q_smem;
+  uint8_t* const v_img = k_img + S::units * S::unit;
+  uint8_t* const stage_img = v_img + S::units * S::unit;
+  uint8_t* const q_img = S::q_smem ? smem : v_img + S::unit;
+  static_assert(S::q_smem != 0 || S::q_tile <= (S::units - 1) * S::unit, "Q in V's units");
 
   constexpr int kConvK = SLOTS * 4, kConvV = kConvK + 4, kMma = kConvV + 4;  // first warps of the roles
   if (warp == kMma) {
     tmem_alloc(&s_tmem, 512);
     if (lane == 0) {
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(&bar.q_full[i], 128);
-        mbar_init(&bar.k_full[i], S::stages == 1 ? 256 : 128);
-        mbar_init(&bar.v_full[i], S::stages == 1 ? 256 : 128);
+      for (int i = 0; i < 4; ++i) {
+        mbar_init(&bar.k_full[i], 128);
+        mbar_init(&bar.v_full[i], 128);
         mbar_init(&bar.k_empty[i], 1);
         mbar_init(&bar.v_empty[i], 1);
         mbar_init(&bar.s_full[i], 2);  // the MMAs, and the issuing thread's own arrival
         mbar_init(&bar.p_full[i], 128);
-        mbar_init(&bar.o_full[i], 1);
       }
-      mbar_init(&bar.pv_done, 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&bar.q_full[i], 128);
+        mbar_init(&bar.pv_done[i], 1);
+        mbar_init(&bar.staged[i], 1);
+      }
       mbar_init(&bar.drained, 1);
-      mbar_init(&bar.staged[0], 1);
-      mbar_init(&bar.staged[1], 1);
       fence_barrier_init();
     }
     tmem_relinquish();
@@ -372,53 +378,76 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
     const uint32_t lanes = tmem + (static_cast<uint32_t>(wq * 32) << 16);
     const uint32_t o_at = lanes + S::o_col + slot * D;
     float m = -INFINITY, l = 0.0f;
-    if (tiles > 0 && sr0 < sr1) {
-      load_q<D>(a, b, h, row0, sr0, sr1, q_img + slot * S::stage, s_down + slot * 128, wq, lane);
-      fence_proxy_async_smem();
-      mbar_arrive(&bar.q_full[slot]);
+    if (units > 0 && sr0 < sr1) {
+      load_q<D>(a, b, h, row0, sr0, sr1, q_img + slot * S::q_tile, s_down + slot * 128, wq, lane);
       __syncwarp();
       const float down = s_down[slot * 128 + wq * 32 + lane];
+      if constexpr (S::q_tmem) {
+        const int qr = wq * 32 + lane;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t x[16];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int at = 4 * c + e;
+            const uint4 v = *reinterpret_cast<const uint4*>(q_img + slot * S::q_tile + (at >> 3) * kQPanel + swizzled(qr, at & 7));
+            x[4 * e] = v.x, x[4 * e + 1] = v.y, x[4 * e + 2] = v.z, x[4 * e + 3] = v.w;
+          }
+          tmem_st16(lanes + S::q_col + slot * (D / 2) + 16 * c, x);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+      } else {
+        fence_proxy_async_smem();
+      }
+      mbar_arrive(&bar.q_full[slot]);
       const int p = len - T + r / a.group;
       const int row_hi = r >= sr1 ? 0 : a.causal ? min(len, p + 1) : len, row_lo = a.window ? p - a.window + 1 : 0;
       // every row of the slot sees the keys [all_lo, all_hi)
       const int all_hi = a.causal ? len - T + sr0 / a.group + 1 : len;
       const int all_lo = a.window ? len - T + (sr1 - 1) / a.group - a.window + 1 : 0;
-      for (int j = 0; j < tiles; ++j) {
-        const int buf = SLOTS == 2 ? slot : j & 1;
-        const uint32_t phase = SLOTS == 2 ? j & 1 : (j >> 1) & 1;
-        if (!warp_wait(&bar.s_full[buf], phase, err, kErrTimeoutAccum)) break;
+      for (int i = 0; i < units; ++i) {
+        const int buf = slot * 2 + (i & 1);
+        const uint32_t s_at = lanes + buf * 64;
+        if (!warp_wait(&bar.s_full[buf], (i >> 1) & 1, err, kErrTimeoutAccum)) break;
         tc_fence_after();
-        const int key0 = keys.lo + j * kKeys;
-        const Tile k{lanes + buf * 128, smem_u32(s_scale[j & 3]), down, row_lo - key0, row_hi - key0};
-        const bool careful = key0 + kKeys > all_hi || key0 < all_lo || s_scale[j & 3][0].w != 0.0f;
-        const float top = careful ? row_max<true>(k, m) : row_max<false>(k, m);
+        uint32_t x[2][32];
+        tmem_ld32(s_at, x[0]);
+        tmem_ld32(s_at + 32, x[1]);
+        const int key0 = keys.lo + i * kKeys;
+        const View k{s_scale[i & 7], down, row_lo - key0, row_hi - key0};
+        const bool careful = key0 + kKeys > all_hi || key0 < all_lo || k.scale[0].w != 0.0f;
+        tmem_ld_wait();
+        const float top = careful ? row_max<true>(k, x, m) : row_max<false>(k, x, m);
         // raise m where it pays; rows of a warp move together
         if (__any_sync(0xffffffffu, top > m + kGrow || (m == -INFINITY && top != -INFINITY))) {
           const float alpha = m == -INFINITY ? 0.0f : ex2(m - top);
-          if (j > 0) {
-            if (SLOTS == 1 && !warp_wait(&bar.pv_done, (j - 1) & 1, err, kErrTimeoutAccum)) break;
+          if (i > 0) {
+            if (!warp_wait(&bar.pv_done[slot], (i - 1) & 1, err, kErrTimeoutAccum)) break;
             tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t x[32];
-              tmem_ld32(o_at + 32 * c, x);
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld16(o_at + 16 * c, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * alpha);
-              tmem_st32(o_at + 32 * c, x);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_st16(o_at + 16 * c, o);
             }
-            tmem_st_wait();
           }
           l *= alpha;
           m = top;
         }
         const float base = m == -INFINITY ? 0.0f : m;
-        l = careful ? row_exp<true>(k, base, l) : row_exp<false>(k, base, l);
+        uint32_t w[2][16];
+        l = careful ? row_exp<true>(k, x, base, l, w) : row_exp<false>(k, x, base, l, w);
+        tmem_st16(s_at, w[0]);
+        tmem_st16(s_at + 16, w[1]);
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&bar.p_full[buf]);
       }
-      warp_wait(&bar.o_full[slot], 0, err, kErrTimeoutAccum);
+      warp_wait(&bar.pv_done[slot], (units - 1) & 1, err, kErrTimeoutAccum);
       tc_fence_after();
     }
     // the rows
@@ -433,7 +462,7 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t x[32];
-        if (tiles > 0) {
+        if (units > 0) {
           tmem_ld32(o_at + 32 * c, x);
           tmem_ld_wait();
         } else {
@@ -467,106 +496,79 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
   } else if (warp < kMma) {
     // ------------------------------------------------------------------------------- codes to f16 images
     if constexpr (S::convert_regs < S::regs) reg_free<S::convert_regs>();
-    // One warpgroup has K, the other V; where there is room for one tile of each only (head_dim 256), both take K and V in
-    // turn: each has to be rewritten while the other is multiplied.  The codes come by bulk copies into a staging tile
-    // (a 16-key group of a head is contiguous in its block), the next one as soon as this one is in registers.
-    constexpr bool kBoth = S::stages == 1;
-    constexpr int kThreads = kBoth ? 256 : 128, kStep = kThreads / (D / 8), kSteps = kKeys / kStep;
-    const bool is_v = !kBoth && warp >= kConvV;
+    constexpr int kStep = 128 / (D / 8), kSteps = kKeys / kStep;
+    const bool is_v = warp >= kConvV;
     const int t = threadIdx.x - (is_v ? kConvV : kConvK) * 32;
     // A thread has chunk c (eight codes, 16 bytes as f16) of the rows row, row + kStep, ...: loads and stores of a
-    // warp are whole rows, without bank conflicts, and the swizzle of its rows is one number (kStep is a multiple of 8).
-    static_assert(kStep % 8 == 0, "swizzle");
+    // warp are whole rows, without bank conflicts.
     const int c = t % (D / 8), row = t / (D / 8);
-    const uint32_t from = smem_u32(stage_img) + (is_v ? kKeys * D : 0) + row * D + c * 8;
-    const uint32_t to = (c >> 3) * kPanel + swizzled(row, c & 7);
-    const bool copies = kBoth ? warp == kConvK : (warp & 3) == 0, scales = warp == kConvK;
+    uint8_t* const stage = stage_img + (is_v ? kKeys * D : 0);
+    const uint32_t from = smem_u32(stage) + row * D + c * 8;
+    const uint32_t to = smem_u32(is_v ? v_img : k_img) + (c >> 3) * kPanel + swizzled(row, c & 7);
+    const bool copies = (warp & 3) == 0, scales = warp == kConvK;
     const int bs_log2 = a.pages.bs_log2, bs = 1 << bs_log2;
     uint64_t* const staged = &bar.staged[is_v ? 1 : 0];
-    // block of the tile's 16-key group `lane` (of eight); -1: none
-    auto ids_of = [&](int j) {
-      const int key = keys.lo + j * kKeys + 16 * (lane & 7);
-      return j < tiles && key < keys.hi ? static_cast<int>(block_of(a.seqs, a.pages, b, key >> bs_log2)) : -1;
+    uint64_t* const full = is_v ? bar.v_full : bar.k_full;
+    uint64_t* const empty = is_v ? bar.v_empty : bar.k_empty;
+    const int8_t* const codes = is_v ? a.pages.v : a.pages.k;
+    // block of the unit's 16-key group `lane` (of four); -1: none
+    auto ids_of = [&](int i) {
+      const int key = keys.lo + i * kKeys + 16 * (lane & 3);
+      return i < units && key < keys.hi ? static_cast<int>(block_of(a.seqs, a.pages, b, key >> bs_log2)) : -1;
     };
-    // groups that there are none of keep the codes that happen to be there: they are hidden, or their scales are NaN
     int issued = 0;
-    auto copy = [&](const int8_t* codes, int j, int id) {
+    // groups that there are none of keep the codes that happen to be there: they are hidden, or their scales are NaN
+    auto copy = [&](int i, int id) {
       ++issued;
-      const bool there = lane < 8 && id >= 0;
+      const bool there = lane < 4 && id >= 0;
       const int n = __popc(__ballot_sync(0xffffffffu, there));
       if (lane == 0) mbar_arrive_expect_tx(staged, n * 16 * D);
       __syncwarp();
       if (there) {
-        const int slot = (keys.lo + j * kKeys + 16 * lane) & (bs - 1);
-        bulk_load(stage_img + (is_v ? kKeys * D : 0) + lane * 16 * D,
-                  codes + (((static_cast<long long>(id) * a.pages.heads + h) << bs_log2) + slot) * D, 16 * D, staged);
+        const int slot = (keys.lo + i * kKeys + 16 * lane) & (bs - 1);
+        bulk_load(stage + lane * 16 * D, codes + (((static_cast<long long>(id) * a.pages.heads + h) << bs_log2) + slot) * D,
+                  16 * D, staged);
       }
     };
-    uint2 raw[kSteps];
-    auto fetch = [&](uint32_t phase) {
-      if (!warp_wait(staged, phase, err, kErrTimeoutFull)) return false;
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) raw[i] = lds64(from + i * kStep * D);
-      named_barrier(is_v ? 2 : 1, kThreads);  // the staging tile is read
-      return true;
-    };
-    auto convert = [&](uint32_t img) {
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        uint32_t u[4];
-        codes_to_half2(raw[i].x, u[0], u[1]);
-        codes_to_half2(raw[i].y, u[2], u[3]);
-        sts128(img + to + i * kStep * 128, u[0], u[1], u[2], u[3]);
-      }
-      fence_proxy_async_smem();
-    };
-    auto wait_empty = [&](uint64_t* empty, int j) {
-      return j < S::stages ||
-             warp_wait(&empty[j % S::stages], ((j / S::stages) - 1) & 1, err, kErrTimeoutEmpty);
-    };
-    const int8_t* const codes = is_v ? a.pages.v : a.pages.k;
-    const uint32_t img = smem_u32(is_v ? v_img : k_img);
     int id = ids_of(0), id_next = ids_of(1);
     RawScales sc{}, sc_next{};
-    if (tiles > 0) {
-      if (copies) copy(codes, 0, id);
+    if (units > 0) {
+      if (copies) copy(0, id);
       if (scales) sc = raw_scales(a, id, h);
     }
     bool ok = true;
-    for (int j = 0; j < tiles && ok; ++j) {
-      const int st = j % S::stages;
-      const int id_after = ids_of(j + 2);
+    for (int i = 0; i < units; ++i) {
+      const int at = i % S::units;
+      const int id_after = ids_of(i + 2);
       if (scales) sc_next = raw_scales(a, id_next, h);
-      if constexpr (kBoth) {
-        ok = fetch(0);
-        if (ok && copies) copy(a.pages.v, j, id);
-        ok = ok && wait_empty(bar.k_empty, j);
-      } else {
-        ok = fetch(j & 1);
-        if (ok && copies && j + 1 < tiles) copy(codes, j + 1, id_next);
-        ok = ok && wait_empty(is_v ? bar.v_empty : bar.k_empty, j);
-      }
+      ok = warp_wait(staged, i & 1, err, kErrTimeoutFull);
+      if (!ok) break;
+      uint2 raw[kSteps];
+#pragma unroll
+      for (int e = 0; e < kSteps; ++e) raw[e] = lds64(from + e * kStep * D);
+      named_barrier(is_v ? 2 : 1, 128);  // the staging tile is read
+      if (copies && i + 1 < units) copy(i + 1, id_next);
+      if (i >= S::units) ok = warp_wait(&empty[at], ((i / S::units) - 1) & 1, err, kErrTimeoutEmpty);
+      if (S::q_smem == 0 && is_v && i == 1) ok = warp_wait(&bar.q_full[0], 0, err, kErrTimeoutEmpty);  // Q has passed
       if (!ok) break;
       if (scales) {
         // .w: a group whose scales need care (zero, or not finite)
         const BlockScales f = fold_scales(a, sc);
         const bool odd = !(f.inv_w < kZeroTile) || !isfinite(f.c);
         const float care = __any_sync(0xffffffffu, odd) ? 1.0f : 0.0f;
-        if (lane < 8) s_scale[j & 3][lane] = make_float4(f.c, f.log2_w, f.inv_w, care);
+        if (lane < 4) s_scale[i & 7][lane] = make_float4(f.c, f.log2_w, f.inv_w, care);
       }
-      if constexpr (kBoth) {
-        convert(img);
-        mbar_arrive(&bar.k_full[0]);
-        ok = fetch(1);
-        if (ok && copies && j + 1 < tiles) copy(a.pages.k, j + 1, id_next);
-        ok = ok && wait_empty(bar.v_empty, j);
-        if (!ok) break;
-        convert(smem_u32(v_img));
-        mbar_arrive(&bar.v_full[0]);
-      } else {
-        convert(img + st * S::stage);
-        mbar_arrive(is_v ? &bar.v_full[st] : &bar.k_full[st]);
+#pragma unroll
+      for (int e = 0; e < kSteps; ++e) {
+        uint32_t u[4];
+        codes_to_half2(raw[e].x, u[0], u[1]);
+        codes_to_half2(raw[e].y, u[2], u[3]);
+        // rows 4 apart (head_dim 256) differ in bit 2 of the swizzle, rows 8 apart not at all
+        const uint32_t flip = kStep == 4 && (e & 1) ? 64u : 0u;
+        sts128((to ^ flip) + at * S::unit + e * kStep * 128, u[0], u[1], u[2], u[3]);
       }
+      fence_proxy_async_smem();
+      mbar_arrive(&full[at]);
       id = id_next, id_next = id_after, sc = sc_next;
     }
     // a wait gave up: copies under way end before the block does
@@ -574,79 +576,57 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
   } else {
     // ------------------------------------------------------------------------------- the MMAs
     reg_free<S::mma_regs>();
-    if (warp == kMma && tiles > 0) {
-      // The whole warp waits and one elected lane issues, so that addresses and descriptors stay in uniform registers:
-      // a lone thread's code moved each of them there per MMA, which took as long as the MMA itself.
+    if (warp == kMma && units > 0) {
       const int slots = SLOTS == 2 && r0 + 128 < r1 ? 2 : 1;
       constexpr uint32_t id_qk = idesc_f16(128, kKeys), id_pv = idesc_f16(128, D, 1);
-      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), leader = elect_one();
       const uint32_t q_desc = desc_lo(smem_u32(q_img), 16), k_desc = desc_lo(smem_u32(k_img), 16),
                      v_desc = desc_lo(smem_u32(v_img), kPanel);
       bool ok = true;
       for (int s = 0; s < slots && ok; ++s) ok = warp_wait(&bar.q_full[s], 0, err, kErrTimeoutFull);
-      auto qk = [&](int s, int buf, int j, bool last) {
-        const uint32_t kd = k_desc + (j % S::stages) * (S::stage >> 4), qd = q_desc + s * (S::stage >> 4);
-        if (elect_one()) {
+      for (int i = 0; i <= units && ok; ++i) {
+        // S of unit i over P of unit i - 2, whose product was issued before
+        if (i < units) {
+          const int at = i % S::units;
+          ok = warp_wait(&bar.k_full[at], (i / S::units) & 1, err, kErrTimeoutFull);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t kd = k_desc + at * (S::unit >> 4);
+          for (int s = 0; s < slots; ++s) {
+            const int buf = s * 2 + (i & 1);
 #pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            constexpr uint32_t step = 32 >> 4, panel = kPanel >> 4;
-            const uint32_t off = (i >> 2) * panel + (i & 3) * step;
-            mma_ss(tm + buf * 128, qd + off, kd + off, id_qk, i != 0);
+            for (int e = 0; e < D / 16; ++e) {
+              const uint32_t b_lo = kd + (e >> 2) * (kPanel >> 4) + (e & 3) * (32 >> 4);
+              if constexpr (S::q_tmem)
+                mma_ts(leader, tm + buf * 64, tm + S::q_col + s * (D / 2) + 8 * e, b_lo, id_qk, e != 0);
+              else
+                mma_ss(leader, tm + buf * 64, q_desc + s * (S::q_tile >> 4) + (e >> 2) * (kQPanel >> 4) + (e & 3) * (32 >> 4),
+                       b_lo, id_qk, e != 0);
+            }
+            commit(leader, smem_u32(&bar.s_full[buf]));
+            arrive(leader, smem_u32(&bar.s_full[buf]));
+            if (s == slots - 1) commit(leader, smem_u32(&bar.k_empty[at]));
           }
-          mma_commit(&bar.s_full[buf]);
-          mbar_arrive(&bar.s_full[buf]);
-          if (last) mma_commit(&bar.k_empty[j % S::stages]);
         }
-        __syncwarp();
-      };
-      auto pv = [&](int s, int buf, int j, bool last) {
-        const uint32_t vd = v_desc + (j % S::stages) * (S::stage >> 4);
-        if (elect_one()) {
-#pragma unroll
-          for (int i = 0; i < kKeys / 16; ++i)
-            mma_ts(tm + S::o_col + s * D, tm + buf * 128 + 8 * i, vd + i * (2048 >> 4), id_pv, j > 0 || i != 0);
-          if (last) mma_commit(&bar.v_empty[j % S::stages]);
-          if (SLOTS == 1) mma_commit(&bar.pv_done);
-          if (j == tiles - 1) mma_commit(&bar.o_full[s]);
-        }
-        __syncwarp();
-      };
-      auto wait_k = [&](int j) { return warp_wait(&bar.k_full[j % S::stages], (j / S::stages) & 1, err, kErrTimeoutFull); };
-      auto wait_v = [&](int j) { return warp_wait(&bar.v_full[j % S::stages], (j / S::stages) & 1, err, kErrTimeoutFull); };
-      for (int j = 0; j <= tiles && ok; ++j) {
-        if constexpr (SLOTS == 2) {
+        if (i > 0) {
+          const int at = (i - 1) % S::units;
+          ok = warp_wait(&bar.v_full[at], ((i - 1) / S::units) & 1, err, kErrTimeoutFull);
+          const uint32_t vd = v_desc + at * (S::unit >> 4);
           for (int s = 0; s < slots && ok; ++s) {
-            if (j > 0) {
-              ok = wait_v(j - 1) && warp_wait(&bar.p_full[s], (j - 1) & 1, err, kErrTimeoutFull);
-              if (!ok) break;
-              tc_fence_after();
-              pv(s, s, j - 1, s == slots - 1);
-            }
-            if (j < tiles) {
-              ok = wait_k(j);
-              if (!ok) break;
-              tc_fence_after();
-              qk(s, s, j, s == slots - 1);
-            }
-          }
-        } else {
-          if (j < tiles) {
-            ok = wait_k(j);
+            const int buf = s * 2 + ((i - 1) & 1);
+            ok = warp_wait(&bar.p_full[buf], ((i - 1) >> 1) & 1, err, kErrTimeoutFull);
             if (!ok) break;
             tc_fence_after();
-            qk(0, j & 1, j, true);
-          }
-          if (j > 0) {
-            ok = wait_v(j - 1) && warp_wait(&bar.p_full[(j - 1) & 1], ((j - 1) >> 1) & 1, err, kErrTimeoutFull);
-            if (!ok) break;
-            tc_fence_after();
-            pv(0, (j - 1) & 1, j - 1, true);
+#pragma unroll
+            for (int e = 0; e < kKeys / 16; ++e)
+              mma_ts(leader, tm + S::o_col + s * D, tm + buf * 64 + 8 * e, vd + e * (2048 >> 4), id_pv, i > 1 || e != 0);
+            commit(leader, smem_u32(&bar.pv_done[s]));
+            if (s == slots - 1) commit(leader, smem_u32(&bar.v_empty[at]));
           }
         }
       }
       if (!ok) {  // a wait gave up: nothing issued here may run on when tensor memory is freed
-        if (elect_one()) mma_commit(&bar.drained);
-        __syncwarp();
+        commit(leader, smem_u32(&bar.drained));
         warp_wait(&bar.drained, 0, err, kErrTimeoutOther);
       }
     }
