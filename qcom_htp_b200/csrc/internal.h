@@ -137,6 +137,9 @@ bool make_tmap_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base,
                   CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B);
 // prepared weight planes: box (tile, K block) at row (tile * kblocks + kb) * b_rows, copied verbatim
 bool make_tmap_planes(CUtensorMap* map, const QhtpMatmulPlan* plan);
+// [tiles][rows][inner] bytes, contiguous, in boxes of box_rows rows of box_inner bytes
+bool make_tmap_tiles_u8(CUtensorMap* map, const void* base, uint64_t inner, uint64_t rows, uint64_t tiles, uint32_t box_inner,
+                        uint32_t box_rows, CUtensorMapSwizzle swizzle);
 bool make_tmap_2d_u8(CUtensorMap* map, const void* base, uint64_t inner, uint64_t rows, uint64_t row_stride_bytes,
                      uint32_t box_inner, uint32_t box_rows);
 

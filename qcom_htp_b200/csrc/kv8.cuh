@@ -197,6 +197,11 @@ __device__ __forceinline__ long long part_rows(const Kv8Attn& a) {
   return static_cast<long long>(a.seqs.batch) * a.pages.heads * a.row_groups * a.chunks * a.tile_rows;
 }
 
+// mbar_wait for a whole warp: every lane goes on, or none does.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
+}
+
 // A block's constants for the softmax: with c = scale * log2(e) * k_scale and w = v_scale, a key's
 // exponent is q . code * c + log2(w), and 1 / w takes w out of the row's sum again.  A v_scale below
 // kScaleMin counts as zero: w is kScaleMin then, and inv_w = kZeroTile tells that the codes add nothing.
@@ -257,9 +262,20 @@ cudaError_t launch_kv8_decode(const Kv8Attn& a);
 // kv8_prompt.cu: rows in tiles of 128 or 256 on tcgen05
 void kv8_prompt_plan(Kv8Attn& a, int sms);
 cudaError_t launch_kv8_prompt(const Kv8Attn& a);
-cudaError_t kv8_read_error(int* code, cudaStream_t stream);
+
 // joins the chunks of a launch
 cudaError_t launch_kv8_combine(const Kv8Attn& a);
+// the current device's error words of the two (a wait that gave up leaves its code), read and cleared; synchronizes
+cudaError_t kv8_prompt_error(int* code, cudaStream_t stream);
+cudaError_t kv8_decode_error(int* code, cudaStream_t stream);
+inline cudaError_t kv8_take_error(const void* symbol, int* code, cudaStream_t stream) {
+  void* at = nullptr;
+  cudaError_t e = cudaGetSymbolAddress(&at, symbol);
+  if (e == cudaSuccess) e = cudaMemcpyAsync(code, at, sizeof(int), cudaMemcpyDeviceToHost, stream);
+  if (e == cudaSuccess) e = cudaMemsetAsync(at, 0, sizeof(int), stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+  return e;
+}
 inline size_t kv8_part_bytes(const Kv8Attn& a) {
   if (a.chunks <= 1) return 0;
   return static_cast<size_t>(a.seqs.batch) * a.pages.heads * a.row_groups * a.chunks * a.tile_rows * (a.head_dim + 2) *

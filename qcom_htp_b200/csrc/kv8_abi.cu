@@ -1,4 +1,5 @@
 // C ABI of the 8-bit KV cache: argument checks and dispatch.
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 
@@ -22,6 +23,7 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 // Shapes only: no pointer is looked at.
 QhtpStatus check_shapes(const QhtpKv8Cache& c, const QhtpKv8Seqs& s) {
   if (c.num_blocks <= 0 || c.kv_heads == 0) return invalid("kv8: the cache needs blocks and heads");
+  if (c.num_blocks > 0x7fffffffll / c.kv_heads) return unsupported("kv8: at most 2^31 - 1 (block, kv head) tiles");
   if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256)
     return unsupported("kv8: head_dim must be 64, 128 or 256");
   if (c.block_size != 16 && c.block_size != 32 && c.block_size != 64 && c.block_size != 128)
@@ -86,9 +88,13 @@ QhtpStatus check_move(const QhtpKv8Move* m, Kv8Move* out) {
   return QHTP_STATUS_OK;
 }
 
+// SMs of the current device, looked up once per device.
 int sm_count() {
+  static std::atomic<int> known[64];
   int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return sms;
+  if (const int n = known[dev].load(std::memory_order_relaxed)) return n;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) known[dev].store(sms);
   return sms;
 }
 
@@ -176,9 +182,12 @@ QhtpStatus qhtp_kv8_attention(const QhtpKv8Attention* run) {
 }
 
 QhtpStatus qhtp_kv8_check(int* device_code, void* stream) {
-  int code = 0;
-  const QhtpStatus st = status_from_cuda(kv8_read_error(&code, static_cast<cudaStream_t>(stream)));
+  int code = 0, other = 0;
+  cudaError_t e = kv8_prompt_error(&code, static_cast<cudaStream_t>(stream));
+  if (e == cudaSuccess) e = kv8_decode_error(&other, static_cast<cudaStream_t>(stream));
+  const QhtpStatus st = status_from_cuda(e);
   if (st != QHTP_STATUS_OK) return st;
+  if (code == 0) code = other;
   if (device_code != nullptr) *device_code = code;
   if (code == 0) return QHTP_STATUS_OK;
   set_last_message("kv8: a wait inside an attention kernel gave up");

@@ -8,11 +8,11 @@
 // loses at most 2^-12 of what it adds to the output.  Scores, maxima, sums and outputs are float32.
 //
 // Bound by memory: two bytes per key and element.  The keys of a (sequence, kv head) are cut into chunks
-// over the grid; a CTA's four warps take 32 keys in turn, straight from global memory to registers in
-// 16-byte loads (a block's tile of a head is contiguous), K of the next step while the softmax of this
-// one runs.  Keys are the M side of the MMAs (m16n8k16, S^T = K Q^T and O^T = V^T P^T), so a group of
-// eight query rows wastes nothing; which head_dim index a fragment's k stands for is free, and is chosen
-// so that a thread's 16 loaded bytes are its fragments.
+// over the grid, a CTA's four warps take 32 of them (16 at head_dim 256) in turn, and each warp keeps a ring of
+// them in shared memory filled by TMA, so that the loads in flight do not hang on registers or on what the warp does.
+// Keys are the M side of the MMAs (m16n8k16, S^T = K Q^T and O^T = V^T P^T), so a group of eight query rows
+// wastes nothing.  Which head_dim index a fragment's k stands for is free: a thread's 16 bytes of a key are its
+// fragments, and with the swizzle that TMA applies neither K's nor V's reads have bank conflicts (V of head_dim 64: two ways).
 #include <algorithm>
 
 #include "kv8.cuh"
@@ -22,8 +22,9 @@ namespace kv8 {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kSeg = 2048;                  // keys whose block constants are in shared memory
-constexpr int kSegBlocks = kSeg / 16 + 2;
+constexpr int kSegBlocks = 256;  // blocks whose constants are in shared memory at a time
+
+__device__ int g_error;          // a wait that gave up leaves its code here
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
@@ -44,21 +45,50 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
-// NT groups of eight rows; K16 groups of 16 keys per step.
-template <int D, int NT, int K16>
-__global__ void __launch_bounds__(kWarps * 32) kv8_decode_kernel(const Kv8Attn a) {
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+  uint4 r;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at) : "memory");
+  return r;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t at) {
+  uint2 r;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(at) : "memory");
+  return r;
+}
+
+// NT groups of eight rows.
+template <int D, int NT>
+struct Ring {
+  static constexpr int k16 = D == 256 || NT == 4 ? 1 : 2;        // 16-key groups of a step
+  static constexpr int box = 16 * (D < 128 ? D : 128);           // bytes of a TMA box: 16 keys of a 128-byte panel
+  static constexpr int panels = D == 256 ? 2 : 1;
+  static constexpr int half = k16 * panels * box;                // K, or V, of a step
+  static constexpr int stages = 16384 / (2 * half);              // 16 KB a warp
+  static constexpr int smem = kWarps * stages * 2 * half + 1024;
+  static_assert(8 * NT * (D + 4) * 4 <= smem - 1024, "the rows are joined in the rings' memory");
+};
+
+template <int D, int NT>
+__global__ void __launch_bounds__(kWarps * 32)
+    kv8_decode_kernel(const Kv8Attn a, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+  using Rg = Ring<D, NT>;
+  constexpr int K16 = Rg::k16;
   constexpr int kRows = 8 * NT;
   constexpr int kQStride = D + 4;      // halves: rows 2 banks apart, so the 64-bit fragment reads do not collide
   constexpr int kOStride = D + 4;
   constexpr int KJ = D / 64;           // 16-byte pieces of a key in one thread
   constexpr int VW = D / 32;           // words of a V row in one thread
   constexpr int MT = D / 16;
+  extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(16) __half s_q[kRows * kQStride];
-  __shared__ __align__(16) float s_o[kRows * kOStride];
   __shared__ float s_down[kRows], s_m[kWarps][kRows], s_l[kWarps][kRows];
   __shared__ int s_lo[kRows], s_hi[kRows];
-  __shared__ long long s_off[kSegBlocks];
+  __shared__ int s_id[kSegBlocks];
   __shared__ float s_c[kSegBlocks], s_lw[kSegBlocks], s_iw[kSegBlocks];
+  __shared__ uint64_t s_full[kWarps][Rg::stages];
+  uint8_t* const ring = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  float* const s_o = reinterpret_cast<float*>(ring);
+  int* const err = &g_error;
 
   const int b = blockIdx.z, h = blockIdx.y, rg = blockIdx.x / a.chunks, chunk = blockIdx.x - rg * a.chunks;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
@@ -75,6 +105,11 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_decode_kernel(const Kv8Attn a
   // each row of the group sees the keys [all_lo, all_hi)
   const int all_hi = a.causal ? len - T + r0 / a.group + 1 : len;
   const int all_lo = a.window ? len - T + (r1 - 1) / a.group - a.window + 1 : 0;
+
+  if (lane < Rg::stages) mbar_init(&s_full[warp][lane], 1);
+  fence_barrier_init();
+  const uint32_t my_ring = smem_u32(ring) + warp * Rg::stages * 2 * Rg::half;
+  uint32_t turn = 0;  // steps of this warp so far: stage turn % stages, phase turn / stages
 
   // the rows of q, each scaled by a power of two into f16
   for (int r = warp; r < kRows; r += kWarps) {
@@ -139,65 +174,44 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_decode_kernel(const Kv8Attn a
   }
 
   const int bs_log2 = a.pages.bs_log2, bs = 1 << bs_log2;
-  for (int seg = keys.lo; seg < keys.hi; seg += kSeg) {
-    const int seg_hi = min(keys.hi, seg + kSeg);
+  const long long seg_keys = static_cast<long long>(kSegBlocks - 1) << bs_log2;  // a segment may start inside a block
+  bool ok = true;
+  for (long long seg0 = keys.lo; seg0 < keys.hi; seg0 += seg_keys) {
+    const int seg = static_cast<int>(seg0), seg_hi = static_cast<int>(min(static_cast<long long>(keys.hi), seg0 + seg_keys));
     const int blk0 = seg >> bs_log2, nblk = ((seg_hi - 1) >> bs_log2) - blk0 + 1;
     for (int i = threadIdx.x; i < nblk; i += kWarps * 32) {
       const long long id = block_of(a.seqs, a.pages, b, blk0 + i);
-      s_off[i] = ((max(id, 0ll) * a.pages.heads + h) << bs_log2) * D;
+      s_id[i] = static_cast<int>(id);
       const BlockScales s = fold_scales(a, raw_scales(a, id, h));
       s_c[i] = s.c, s_lw[i] = s.log2_w, s_iw[i] = s.inv_w;
     }
     __syncthreads();
 
     const int groups = (seg_hi - seg + 15) >> 4, tiles = (groups + K16 - 1) / K16;
-    uint4 kr[K16][2][KJ];
-    uint32_t vr[K16][4][VW];
-    auto place = [&](int gi, long long& off) {  // block index in the segment, and the group's first code
-      const int key = seg + min(gi, groups - 1) * 16, bi = (key >> bs_log2) - blk0;
-      off = s_off[bi] + static_cast<long long>(key & (bs - 1)) * D;
-      return bi;
-    };
-    auto load_k = [&](int tile) {
-#pragma unroll
-      for (int i = 0; i < K16; ++i) {
-        long long off;
-        place(tile * K16 + i, off);
-        const int8_t* p = a.pages.k + off + g * D + 16 * q4;
-#pragma unroll
-        for (int j = 0; j < KJ; ++j) {
-          kr[i][0][j] = __ldg(reinterpret_cast<const uint4*>(p + 64 * j));
-          kr[i][1][j] = __ldg(reinterpret_cast<const uint4*>(p + 8 * D + 64 * j));
-        }
+    auto block_at = [&](int gi) { return ((seg + min(gi, groups - 1) * 16) >> bs_log2) - blk0; };
+    // A lane per box: K and V, groups, panels.  A group that is not there, or that the table does not map, is not
+    // copied: its codes are whatever the ring holds, and its keys are hidden or their scales NaN.
+    auto copy = [&](int tile, uint32_t at) {
+      constexpr int kBoxes = 2 * K16 * Rg::panels;
+      const int st = at % Rg::stages, gi = tile * K16 + (lane / 2) % K16, panel = lane / (2 * K16);
+      const int key = seg + gi * 16;
+      const int id = lane < kBoxes && gi < groups ? s_id[block_at(gi)] : -1;
+      const int n = __popc(__ballot_sync(0xffffffffu, id >= 0));
+      if (lane == 0) mbar_arrive_expect_tx(&s_full[warp][st], n * Rg::box);
+      __syncwarp();
+      if (id >= 0) {
+        const uint32_t to = my_ring + st * 2 * Rg::half + (lane & 1) * Rg::half + ((lane / 2) % K16 * Rg::panels + panel) * Rg::box;
+        tma_load_3d(to, lane & 1 ? &map_v : &map_k, smem_u32(&s_full[warp][st]), panel * 128, key & (bs - 1),
+                    static_cast<int>(id * static_cast<long long>(a.pages.heads) + h));
       }
     };
-    auto load_v = [&](int tile) {
-#pragma unroll
-      for (int i = 0; i < K16; ++i) {
-        long long off;
-        place(tile * K16 + i, off);
-        const int8_t* p = a.pages.v + off + (D / 8) * g;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int8_t* row = p + (2 * q4 + (x & 1) + 8 * (x >> 1)) * D;
-          if constexpr (VW == 2) {
-            const uint2 v = __ldg(reinterpret_cast<const uint2*>(row));
-            vr[i][x][0] = v.x, vr[i][x][1] = v.y;
-          } else {
-#pragma unroll
-            for (int w = 0; w < VW; w += 4) {
-              const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + 4 * w));
-              vr[i][x][w] = v.x, vr[i][x][w + 1] = v.y, vr[i][x][w + 2] = v.z, vr[i][x][w + 3] = v.w;
-            }
-          }
-        }
-      }
-    };
-    if (warp < tiles) {
-      load_k(warp);
-      load_v(warp);
-    }
-    for (int tile = warp; tile < tiles; tile += kWarps) {
+    const uint32_t turn0 = turn;
+    for (int i = 0; i < Rg::stages; ++i)
+      if (warp + i * kWarps < tiles) copy(warp + i * kWarps, turn0 + i);
+    for (int tile = warp; tile < tiles && ok; tile += kWarps, ++turn) {
+      ok = warp_wait(&s_full[warp][turn % Rg::stages], (turn / Rg::stages) & 1, err, kErrTimeoutFull);
+      if (!ok) break;
+      const uint32_t k_at = my_ring + (turn % Rg::stages) * 2 * Rg::half, v_at = k_at + Rg::half;
       // S^T = K Q^T
       float s[K16][NT][4];
 #pragma unroll
@@ -208,16 +222,27 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_decode_kernel(const Kv8Attn a
           for (int e = 0; e < 4; ++e) s[i][n][e] = 0.0f;
 #pragma unroll
       for (int j = 0; j < KJ; ++j) {
+        uint4 kr[K16][2];
+#pragma unroll
+        for (int i = 0; i < K16; ++i)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int row = g + 8 * r;
+            const uint32_t box = k_at + (i * Rg::panels + (j >> 1)) * Rg::box;
+            kr[i][r] = lds128(D == 64 ? box + row * 64 + ((q4 ^ ((row >> 1) & 3)) << 4)
+                                      : box + row * 128 + (((2 * q4 + (j & 1)) ^ (row & 7)) << 4));
+          }
+        const int d0 = D == 64 ? 16 * q4 : 128 * (j >> 1) + 32 * q4 + 16 * (j & 1);  // head_dim of the piece
 #pragma unroll
         for (int st = 0; st < 4; ++st) {
           uint2 qf[NT];
 #pragma unroll
           for (int n = 0; n < NT; ++n)
-            qf[n] = *reinterpret_cast<const uint2*>(&s_q[(8 * n + g) * kQStride + 64 * j + 16 * q4 + 4 * st]);
+            qf[n] = *reinterpret_cast<const uint2*>(&s_q[(8 * n + g) * kQStride + d0 + 4 * st]);
 #pragma unroll
           for (int i = 0; i < K16; ++i) {
-            const uint32_t w0 = reinterpret_cast<const uint32_t*>(&kr[i][0][j])[st];
-            const uint32_t w1 = reinterpret_cast<const uint32_t*>(&kr[i][1][j])[st];
+            const uint32_t w0 = reinterpret_cast<const uint32_t*>(&kr[i][0])[st];
+            const uint32_t w1 = reinterpret_cast<const uint32_t*>(&kr[i][1])[st];
             uint32_t a0, a1, a2, a3;
             codes_to_half2(w0, a0, a2);
             codes_to_half2(w1, a1, a3);
@@ -226,7 +251,6 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_decode_kernel(const Kv8Attn a
           }
         }
       }
-      if (tile + kWarps < tiles) load_k(tile + kWarps);
 
       const int key0 = seg + tile * 16 * K16;
       const bool masked = key0 + 16 * K16 > all_hi || key0 < all_lo;
@@ -236,8 +260,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_decode_kernel(const Kv8Attn a
       for (int n = 0; n < NT; ++n) top[n][0] = m[n][0], top[n][1] = m[n][1];
 #pragma unroll
       for (int i = 0; i < K16; ++i) {
-        long long off;
-        const int bi = place(tile * K16 + i, off);
+        const int bi = block_at(tile * K16 + i);
         const float c = s_c[bi], lw = s_lw[bi];
         iw[i] = s_iw[bi];
         zero[i] = iw[i] == kZeroTile;
@@ -288,12 +311,28 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_decode_kernel(const Kv8Attn a
       // O^T += V^T P^T
 #pragma unroll
       for (int i = 0; i < K16; ++i) {
+        uint32_t vr[4][VW];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int row = 2 * q4 + (x & 1) + 8 * (x >> 1);
+          const uint32_t box = v_at + i * Rg::panels * Rg::box;
+          if constexpr (D == 64) {
+            const uint2 v = lds64(box + row * 64 + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + (g & 1) * 8);
+            vr[x][0] = v.x, vr[x][1] = v.y;
+          } else {
+#pragma unroll
+            for (int w = 0; w < VW; w += 4) {
+              const uint4 v = lds128(box + (w >> 2) * Rg::box + row * 128 + ((g ^ (row & 7)) << 4));
+              vr[x][w] = v.x, vr[x][w + 1] = v.y, vr[x][w + 2] = v.z, vr[x][w + 3] = v.w;
+            }
+          }
+        }
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
           uint32_t x[2][4];  // [key pair][element of the word]
 #pragma unroll
           for (int kp = 0; kp < 2; ++kp) {
-            const uint32_t u0 = vr[i][2 * kp][w] ^ 0x80808080u, u1 = vr[i][2 * kp + 1][w] ^ 0x80808080u;
+            const uint32_t u0 = vr[2 * kp][w] ^ 0x80808080u, u1 = vr[2 * kp + 1][w] ^ 0x80808080u;
             const uint32_t lo = prmt(u0, u1, 0x5140u), hi = prmt(u0, u1, 0x7362u);
             x[kp][0] = sub_1152(prmt(lo, 0x64646464u, 0x4140u));
             x[kp][1] = sub_1152(prmt(lo, 0x64646464u, 0x4342u));
@@ -307,9 +346,17 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_decode_kernel(const Kv8Attn a
           }
         }
       }
-      if (tile + kWarps < tiles) load_v(tile + kWarps);
+      __syncwarp();  // the stage is read
+      if (tile + Rg::stages * kWarps < tiles) copy(tile + Rg::stages * kWarps, turn + Rg::stages);
     }
-    __syncthreads();  // the segment's constants are read
+    if (!ok) {  // a wait gave up: what is under way lands before the block ends
+      const uint32_t last = turn0 + (tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0);
+      for (uint32_t i = 0; i < Rg::stages && turn + i < last; ++i)
+        warp_wait(&s_full[warp][(turn + i) % Rg::stages], ((turn + i) / Rg::stages) & 1, err, kErrTimeoutOther);
+      ok = false;
+    }
+    __syncthreads();  // the segment's constants, and the rings, are read
+    if (!__syncthreads_and(ok)) break;
   }
 
   // join the warps: every row's maximum, then the rows added up one warp after the other
@@ -333,12 +380,13 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_decode_kernel(const Kv8Attn a
 #pragma unroll
           for (int x = 1; x < kWarps; ++x) top = fmaxf(top, s_m[x][r]);
           const float alpha = ex2(m[n][i] - (top == -INFINITY ? 0.0f : top));
-          float* o = s_o + r * kOStride + (D / 8) * g;
+          float* o = s_o + r * kOStride;
 #pragma unroll
           for (int t = 0; t < MT; ++t) {
             const float x0 = acc[n][t][i] * alpha, x1 = acc[n][t][i + 2] * alpha;
-            o[2 * t] = w ? o[2 * t] + x0 : x0;
-            o[2 * t + 1] = w ? o[2 * t + 1] + x1 : x1;
+            const int d = D == 64 ? 8 * g + 2 * t : 128 * (t >> 3) + 16 * g + 2 * (t & 7);
+            o[d] = w ? o[d] + x0 : x0;
+            o[d + 1] = w ? o[d + 1] + x1 : x1;
           }
         }
     }
@@ -410,10 +458,20 @@ __global__ void __launch_bounds__(128) kv8_combine_kernel(const Kv8Attn a) {
   write_row8(a, b, row0, row, h, 8 * c, o, sum, top);
 }
 
-template <int D, int NT, int K16>
+template <int D, int NT>
 cudaError_t run(const Kv8Attn& a) {
+  using Rg = Ring<D, NT>;
+  CUtensorMap map[2];
+  const uint64_t tiles = static_cast<uint64_t>(a.pages.num_blocks) * a.pages.heads;
+  const CUtensorMapSwizzle swizzle = D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+  for (int i = 0; i < 2; ++i)
+    if (!make_tmap_tiles_u8(&map[i], i ? a.pages.v : a.pages.k, D, 1ull << a.pages.bs_log2, tiles, D < 128 ? D : 128, 16, swizzle))
+      return cudaErrorInvalidValue;
+  const cudaError_t e =
+      cudaFuncSetAttribute(kv8_decode_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Rg::smem);
+  if (e != cudaSuccess) return e;
   const dim3 grid(static_cast<unsigned>(a.chunks) * a.row_groups, a.pages.heads, a.seqs.batch);
-  kv8_decode_kernel<D, NT, K16><<<grid, kWarps * 32, 0, a.stream>>>(a);
+  kv8_decode_kernel<D, NT><<<grid, kWarps * 32, Rg::smem, a.stream>>>(a, map[0], map[1]);
   return cudaGetLastError();
 }
 
@@ -456,14 +514,14 @@ void kv8_decode_plan(Kv8Attn& a, int sms) {
 
 cudaError_t launch_kv8_decode(const Kv8Attn& a) {
   switch (a.head_dim * 100 + a.tile_rows) {
-    case 6408: return kv8::run<64, 1, 2>(a);
-    case 6416: return kv8::run<64, 2, 2>(a);
-    case 6432: return kv8::run<64, 4, 2>(a);
-    case 12808: return kv8::run<128, 1, 2>(a);
-    case 12816: return kv8::run<128, 2, 2>(a);
-    case 12832: return kv8::run<128, 4, 1>(a);
-    case 25608: return kv8::run<256, 1, 1>(a);
-    case 25616: return kv8::run<256, 2, 1>(a);
+    case 6408: return kv8::run<64, 1>(a);
+    case 6416: return kv8::run<64, 2>(a);
+    case 6432: return kv8::run<64, 4>(a);
+    case 12808: return kv8::run<128, 1>(a);
+    case 12816: return kv8::run<128, 2>(a);
+    case 12832: return kv8::run<128, 4>(a);
+    case 25608: return kv8::run<256, 1>(a);
+    case 25616: return kv8::run<256, 2>(a);
     default: return cudaErrorInvalidValue;
   }
 }
@@ -473,5 +531,7 @@ cudaError_t launch_kv8_combine(const Kv8Attn& a) {
   if (a.head_dim == 128) return kv8::combine<128>(a);
   return kv8::combine<256>(a);
 }
+
+cudaError_t kv8_decode_error(int* code, cudaStream_t stream) { return kv8_take_error(&kv8::g_error, code, stream); }
 
 }  // namespace qhtp

@@ -121,6 +121,12 @@ __device__ __forceinline__ float2 ex2_poly(float2 t) {
   return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(big.x) << 23)),
                      __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(big.y) << 23)));
 }
+// Keeps uses of what tcgen05.ld wrote behind the wait for it: the wait itself does not name the registers.
+template <int N>
+__device__ __forceinline__ void pin(uint32_t (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(x[i]));
+}
 __device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -229,11 +235,6 @@ __device__ __forceinline__ void load_q(const Kv8Attn& a, int b, int h, long long
 
 // The word that a wait of a kernel here, having given up, leaves its code in.
 __device__ int g_error;
-
-// mbar_wait for a whole warp: every lane goes on, or none does.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int code) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
-}
 
 // A row's view of a unit: the group constants, and the columns that the row sees.  CAREFUL below: the unit has columns
 // that not every row sees, or a group whose scales are not plain.
@@ -418,6 +419,7 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
         const View k{s_scale[i & 7], down, row_lo - key0, row_hi - key0};
         const bool careful = key0 + kKeys > all_hi || key0 < all_lo || k.scale[0].w != 0.0f;
         tmem_ld_wait();
+        pin(x[0]), pin(x[1]);
         const float top = careful ? row_max<true>(k, x, m) : row_max<false>(k, x, m);
         // raise m where it pays; rows of a warp move together
         if (__any_sync(0xffffffffu, top > m + kGrow || (m == -INFINITY && top != -INFINITY))) {
@@ -430,6 +432,7 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
               uint32_t o[16];
               tmem_ld16(o_at + 16 * c, o);
               tmem_ld_wait();
+              pin(o);
 #pragma unroll
               for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
               tmem_st16(o_at + 16 * c, o);
@@ -447,6 +450,9 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
         tc_fence_before();
         mbar_arrive(&bar.p_full[buf]);
       }
+      // the last product may be two phases ahead of what this warp has seen (S of a unit comes before P V of the one before
+      // it), and a parity tells only one: both are waited for
+      if (units > 1) warp_wait(&bar.pv_done[slot], (units - 2) & 1, err, kErrTimeoutAccum);
       warp_wait(&bar.pv_done[slot], (units - 1) & 1, err, kErrTimeoutAccum);
       tc_fence_after();
     }
@@ -465,6 +471,7 @@ __global__ void __launch_bounds__(Shape<D, SLOTS>::threads, 1) kv8_prompt_kernel
         if (units > 0) {
           tmem_ld32(o_at + 32 * c, x);
           tmem_ld_wait();
+          pin(x);
         } else {
 #pragma unroll
           for (int e = 0; e < 32; ++e) x[e] = 0;
@@ -688,13 +695,6 @@ cudaError_t launch_kv8_prompt(const Kv8Attn& a) {
   }
 }
 
-cudaError_t kv8_read_error(int* code, cudaStream_t stream) {
-  void* at = nullptr;
-  cudaError_t e = cudaGetSymbolAddress(&at, kv8::g_error);
-  if (e == cudaSuccess) e = cudaMemcpyAsync(code, at, sizeof(int), cudaMemcpyDeviceToHost, stream);
-  if (e == cudaSuccess) e = cudaMemsetAsync(at, 0, sizeof(int), stream);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
-  return e;
-}
+cudaError_t kv8_prompt_error(int* code, cudaStream_t stream) { return kv8_take_error(&kv8::g_error, code, stream); }
 
 }  // namespace qhtp

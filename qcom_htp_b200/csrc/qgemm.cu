@@ -74,6 +74,20 @@ bool make_tmap_2d_u8(CUtensorMap* map, const void* base, uint64_t inner, uint64_
   return make_tmap_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, inner, rows, row_stride_bytes, box_inner, box_rows);
 }
 
+// [tiles][rows][inner] bytes, contiguous; box: box_rows rows of box_inner bytes of one tile.
+bool make_tmap_tiles_u8(CUtensorMap* map, const void* base, uint64_t inner, uint64_t rows, uint64_t tiles, uint32_t box_inner,
+                        uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+  PFN_encodeTiled enc = get_encode_fn();
+  if (enc == nullptr) return false;
+  cuuint64_t dims[3] = {inner, rows, tiles};
+  cuuint64_t strides[2] = {inner, inner * rows};
+  cuuint32_t box[3] = {box_inner, box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // The prepared weight planes as [n_tiles * kblocks * b_rows, 128] bytes: each (tile, K block) is one
 // contiguous, already swizzled operand image, copied verbatim (no TMA swizzle) into a stage.
 bool make_tmap_planes(CUtensorMap* map, const QhtpMatmulPlan* plan) {

@@ -63,7 +63,7 @@ def attention(**kw):
 SHAPES = [(dict(cache=cache(num_blocks=0)), L.INVALID_ARGUMENT), (dict(cache=cache(kv_heads=0)), L.INVALID_ARGUMENT),
           (dict(cache=cache(head_dim=96)), L.UNSUPPORTED), (dict(cache=cache(block_size=48)), L.UNSUPPORTED),
           (dict(cache=cache(block_size=8)), L.UNSUPPORTED), (dict(seqs=seqs(batch=65536)), L.UNSUPPORTED),
-          (dict(seqs=seqs(total=-1)), L.INVALID_ARGUMENT), (dict(seqs=seqs(max_blocks=1 << 28)), L.UNSUPPORTED),
+          (dict(cache=cache(num_blocks=1 << 30)), L.UNSUPPORTED), (dict(seqs=seqs(total=-1)), L.INVALID_ARGUMENT), (dict(seqs=seqs(max_blocks=1 << 28)), L.UNSUPPORTED),
           (dict(cache=cache(k=0)), L.INVALID_ARGUMENT), (dict(cache=cache(v_scale=0)), L.INVALID_ARGUMENT),
           (dict(cache=cache(v=8)), L.INVALID_ARGUMENT), (dict(seqs=seqs(block_table=0)), L.INVALID_ARGUMENT)]
 

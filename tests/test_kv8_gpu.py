@@ -351,6 +351,22 @@ def test_runs_repeat_bit_for_bit():
         assert torch.equal(x[0], a[0][0]) and torch.equal(x[1], a[0][1])
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("lengths,t,hq,bs", [([200, 333], 200, 4, 64), ([2000, 1333, 1000], 150, 16, 16), ([4000] * 9, 1, 8, 32)])
+def test_many_runs_give_the_same_bits(d, lengths, t, hq, bs):
+    """The kernels' roles hand over through barriers: none may depend on who comes first."""
+    blocks = sum(-(-n // bs) for n in lengths)
+    cache = random_cache(blocks, 2, d, bs, 1)
+    table, n = i32(random_table(lengths, bs, blocks, 2)), i32(lengths)
+    q = torch.randn((len(lengths), t, hq, d), device="cuda", dtype=BF)
+    busy = torch.randn((1024, 1024), device="cuda")
+    first = qhtp.kv8_attention(q, cache, table, n)
+    for i in range(80):
+        if i % 3 == 0:
+            busy @ busy
+        assert torch.equal(qhtp.kv8_attention(q, cache, table, n), first), i
+
+
 def test_on_another_stream():
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
