@@ -421,41 +421,118 @@ __global__ void __launch_bounds__(kWarps * 32)
   }
 }
 
-// The chunks of each row joined: D / 8 threads a row, 128 / (D / 8) rows of a (sequence, kv head) a CTA.
+constexpr int kFew = 8;
+
+// Chunks that a row group's keys fill: those that its attention kernel wrote.
+__device__ __forceinline__ int chunks_used(const Kv8Attn& a, const Span& s) {
+  const long long span = s.hi - (s.lo & ~31);
+  return span <= 0 ? 1 : static_cast<int>(min(static_cast<long long>(a.chunks), (span + a.chunk - 1) / a.chunk));
+}
+
+// The chunks of each row joined, few of them: D / 8 threads a row, each over all chunks.
 template <int D>
-__global__ void __launch_bounds__(128) kv8_combine_kernel(const Kv8Attn a) {
-  constexpr int kLanes = D / 8;                 // threads of a row
-  constexpr int kPer = 128 / kLanes;            // rows of a CTA
+__global__ void __launch_bounds__(128) kv8_combine_few_kernel(const Kv8Attn a) {
+  constexpr int kLanes = D / 8, kPer = 128 / kLanes;
   griddep_wait();
   const int b = blockIdx.z, h = blockIdx.y, row = blockIdx.x * kPer + threadIdx.x / kLanes, c = threadIdx.x % kLanes;
   long long row0;
   const int T = seq_rows(a.seqs, b, row0);
   const int R = T * a.group, rg = row / a.tile_rows, r0 = rg * a.tile_rows, r1 = min(R, r0 + a.tile_rows), r = row - r0;
   if (row >= R || rg >= a.row_groups) return;
-  const Span all = row_span(a, seq_length(a, b), T, r0, r1);
-  int n = 1;
-  while (n < a.chunks && chunk_span(a, all, n).lo < chunk_span(a, all, n).hi) ++n;
+  const int n = chunks_used(a, row_span(a, seq_length(a, b), T, r0, r1));
   const long long part = part_row(a, b, h, rg, 0) + r;
-  const float* ml = a.part + part_rows(a) * D;
-  float top = -INFINITY;
-  for (int i = 0; i < n; ++i) {
-    const long long p = part + static_cast<long long>(i) * a.tile_rows;
-    if (ml[2 * p + 1] != 0.0f) top = fmaxf(top, ml[2 * p]);
+  const float* const ml = a.part + part_rows(a) * D;
+  float top = -INFINITY, l[kFew], m[kFew];
+#pragma unroll
+  for (int i = 0; i < kFew; ++i) {
+    const float2 v = i < n ? *reinterpret_cast<const float2*>(ml + 2 * (part + static_cast<long long>(i) * a.tile_rows))
+                           : make_float2(0.0f, 0.0f);
+    m[i] = v.x, l[i] = v.y;
+    if (v.y != 0.0f) top = fmaxf(top, v.x);
   }
   if (top == -INFINITY) top = 0.0f;
   float sum = 0.0f, o[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) {
-    const long long p = part + static_cast<long long>(i) * a.tile_rows;
-    const float l = ml[2 * p + 1];
-    const float f = l != 0.0f ? ex2(ml[2 * p] - top) : 0.0f;
-    const float4* x = reinterpret_cast<const float4*>(a.part + p * D + 8 * c);
+#pragma unroll
+  for (int i = 0; i < kFew; ++i) {
+    if (i >= n) break;
+    const float4* x = reinterpret_cast<const float4*>(a.part + (part + static_cast<long long>(i) * a.tile_rows) * D + 8 * c);
     const float4 u = x[0], v = x[1];
-    sum = fmaf(l, f, sum);
+    const float f = l[i] != 0.0f ? ex2(m[i] - top) : 0.0f;
+    sum = fmaf(l[i], f, sum);
     o[0] = fmaf(u.x, f, o[0]), o[1] = fmaf(u.y, f, o[1]), o[2] = fmaf(u.z, f, o[2]), o[3] = fmaf(u.w, f, o[3]);
     o[4] = fmaf(v.x, f, o[4]), o[5] = fmaf(v.y, f, o[5]), o[6] = fmaf(v.z, f, o[6]), o[7] = fmaf(v.w, f, o[7]);
   }
   write_row8(a, b, row0, row, h, 8 * c, o, sum, top);
+}
+
+// The chunks of a row joined: a CTA a row.  Its threads take the chunks' maxima and sums at once, then each eight
+// elements of every kGroups-th chunk; the groups are added up in their order.
+template <int D>
+__global__ void __launch_bounds__(256) kv8_combine_kernel(const Kv8Attn a) {
+  constexpr int kLanes = D / 8, kGroups = 256 / kLanes, kWeights = 256;
+  __shared__ float s_w[kWeights], s_top[8], s_sum[8];
+  __shared__ float s_o[kGroups][D + 4];
+  griddep_wait();
+  const int b = blockIdx.z, h = blockIdx.y, row = blockIdx.x, t = threadIdx.x;
+  long long row0;
+  const int T = seq_rows(a.seqs, b, row0);
+  const int R = T * a.group, rg = row / a.tile_rows, r0 = rg * a.tile_rows, r1 = min(R, r0 + a.tile_rows), r = row - r0;
+  if (row >= R || rg >= a.row_groups) return;
+  const int n = chunks_used(a, row_span(a, seq_length(a, b), T, r0, r1));
+  const long long part = part_row(a, b, h, rg, 0) + r;
+  const float* const ml = a.part + part_rows(a) * D;
+  auto at = [&](int i) { return part + static_cast<long long>(i) * a.tile_rows; };
+  // the row's maximum over the chunks that saw a key of it
+  float top = -INFINITY;
+  for (int i = t; i < n; i += 256) {
+    const float2 v = *reinterpret_cast<const float2*>(ml + 2 * at(i));
+    if (v.y != 0.0f) top = fmaxf(top, v.x);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if ((t & 31) == 0) s_top[t >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, s_top[i]);
+  if (top == -INFINITY) top = 0.0f;
+
+  const int c = t % kLanes, group = t / kLanes;
+  float sum = 0.0f, o[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+  for (int base = 0; base < n; base += kWeights) {
+    const int m = min(kWeights, n - base);
+    if (t < m) {
+      const float2 v = *reinterpret_cast<const float2*>(ml + 2 * at(base + t));
+      const float w = v.y != 0.0f ? ex2(v.x - top) : 0.0f;
+      s_w[t] = w;
+      sum = fmaf(v.y, w, sum);
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int i = group; i < m; i += kGroups) {
+      const float4* x = reinterpret_cast<const float4*>(a.part + at(base + i) * D + 8 * c);
+      const float4 u = x[0], v = x[1];
+      const float f = s_w[i];
+      o[0] = fmaf(u.x, f, o[0]), o[1] = fmaf(u.y, f, o[1]), o[2] = fmaf(u.z, f, o[2]), o[3] = fmaf(u.w, f, o[3]);
+      o[4] = fmaf(v.x, f, o[4]), o[5] = fmaf(v.y, f, o[5]), o[6] = fmaf(v.z, f, o[6]), o[7] = fmaf(v.w, f, o[7]);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+  if ((t & 31) == 0) s_sum[t >> 5] = sum;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s_o[group][8 * c + e] = o[e];
+  __syncthreads();
+  if (t >= kLanes) return;
+  sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum += s_sum[i];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    o[e] = 0.0f;
+    for (int i = 0; i < kGroups; ++i) o[e] += s_o[i][8 * t + e];
+  }
+  write_row8(a, b, row0, row, h, 8 * t, o, sum, top);
 }
 
 template <int D, int NT>
@@ -477,17 +554,19 @@ cudaError_t run(const Kv8Attn& a) {
 
 template <int D>
 cudaError_t combine(const Kv8Attn& a) {
-  const int per = 128 / (D / 8);
+  const long long rows = static_cast<long long>(a.seqs.tokens) * a.group;
+  const bool few = a.chunks <= kFew;
+  const int per = few ? 128 / (D / 8) : 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<long long>(a.seqs.tokens) * a.group + per - 1) / per), a.pages.heads, a.seqs.batch);
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3(static_cast<unsigned>((rows + per - 1) / per), a.pages.heads, a.seqs.batch);
+  cfg.blockDim = dim3(few ? 128 : 256);
   cfg.stream = a.stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv8_combine_kernel<D>, a);
+  return few ? cudaLaunchKernelEx(&cfg, kv8_combine_few_kernel<D>, a) : cudaLaunchKernelEx(&cfg, kv8_combine_kernel<D>, a);
 }
 
 }  // namespace
@@ -503,13 +582,20 @@ void kv8_decode_plan(Kv8Attn& a, int sms) {
   long long span = a.max_len;
   if (a.window) span = std::min(span, static_cast<long long>(a.window) + a.tile_rows + 31);
   span = std::max(span, 1ll);
-  // Chunks fill three CTAs an SM twice over, of 256 keys at the least and 2048 at the most: the larger the
-  // chunk the less is spent on its start and its join, the smaller the better sequences of unlike lengths
-  // share the SMs.
-  long long chunk = (span * tiles + 6ll * sms - 1) / (6ll * sms);
-  chunk = (std::max(256ll, std::min(2048ll, chunk)) + 127) / 128 * 128;
-  a.chunks = static_cast<int>((span + chunk - 1) / chunk);
+  // Three CTAs fit an SM.  Where the row groups alone are many waves of those, chunks of kMost keys are short enough for
+  // sequences of unlike lengths to share the SMs.  Else the keys are cut so that the CTAs are one whole wave.  Short
+  // spans are left whole: a CTA takes 512 keys in less time than a second kernel needs to join two parts.
+  // Measured, 2 x 131072 keys: one wave 95.6 us, two 103.2, three 109.3, chunks of 2048 keys (2.3 waves) 110.
+  constexpr long long kMost = 2048, kLeast = 256, kWhole = 768;
+  const long long slots = 3ll * sms;
+  long long n = 1;
+  if (span > kWhole) {
+    n = (span + kMost - 1) / kMost;
+    if (n * tiles < 4 * slots) n = std::max(1ll, std::min(slots / tiles, span / kLeast));
+  }
+  const long long chunk = ((span + n - 1) / n + 127) / 128 * 128;
   a.chunk = static_cast<int>(chunk);
+  a.chunks = static_cast<int>((span + chunk - 1) / chunk);
 }
 
 cudaError_t launch_kv8_decode(const Kv8Attn& a) {
