@@ -65,7 +65,7 @@ struct Ring {
   static constexpr int half = k16 * panels * box;                // K, or V, of a step
   static constexpr int stages = 16384 / (2 * half);              // 16 KB a warp
   static constexpr int smem = kWarps * stages * 2 * half + 1024;
-  static_assert(8 * NT * (D + 4) * 4 <= smem - 1024, "the rows are joined in the rings' memory");
+  static_assert(2 * 8 * NT * (D + 4) * 4 <= smem - 1024, "the rows are joined in the rings' memory");
 };
 
 template <int D, int NT>
@@ -106,67 +106,41 @@ __global__ void __launch_bounds__(kWarps * 32)
   const int all_hi = a.causal ? len - T + r0 / a.group + 1 : len;
   const int all_lo = a.window ? len - T + (r1 - 1) / a.group - a.window + 1 : 0;
 
+  if (threadIdx.x == 0) tma_prefetch_desc(&map_k), tma_prefetch_desc(&map_v);
   if (lane < Rg::stages) mbar_init(&s_full[warp][lane], 1);
   fence_barrier_init();
   const uint32_t my_ring = smem_u32(ring) + warp * Rg::stages * 2 * Rg::half;
   uint32_t turn = 0;  // steps of this warp so far: stage turn % stages, phase turn / stages
 
-  // the rows of q, each scaled by a power of two into f16
-  for (int r = warp; r < kRows; r += kWarps) {
-    constexpr int E = D / 32;  // elements of a lane
-    float x[E];
-    const int row = r0 + r;
-    const bool live = row < r1;
-    if (live) {
-      const long long at = b * a.q.batch_stride + (row0 + row / a.group) * a.q.token_stride +
-                           (static_cast<long long>(h) * a.group + row % a.group) * a.q.head_stride + lane * E;
-      const uint16_t* src = static_cast<const uint16_t*>(a.q.data) + at;
-      uint32_t w[(E + 1) / 2];
+  // q's rows are on their way (and, below, the first keys) before anything is done with them
+  constexpr int E = D / 32, kMine = kRows / kWarps;  // elements of a lane, rows of a warp
+  uint32_t qw[kMine][E / 2];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int row = r0 + warp + i * kWarps;
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) qw[i][e] = 0;
+    if (row < r1) {
+      const int t = row / a.group;
+      const uint16_t* src = static_cast<const uint16_t*>(a.q.data) + b * a.q.batch_stride + (row0 + t) * a.q.token_stride +
+                            (static_cast<long long>(h) * a.group + row - t * a.group) * a.q.head_stride + lane * E;
       if constexpr (E == 8) {
         const uint4 v = __ldg(reinterpret_cast<const uint4*>(src));
-        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+        qw[i][0] = v.x, qw[i][1] = v.y, qw[i][2] = v.z, qw[i][3] = v.w;
       } else if constexpr (E == 4) {
         const uint2 v = __ldg(reinterpret_cast<const uint2*>(src));
-        w[0] = v.x, w[1] = v.y;
+        qw[i][0] = v.x, qw[i][1] = v.y;
       } else {
-        w[0] = __ldg(reinterpret_cast<const uint32_t*>(src));
+        qw[i][0] = __ldg(reinterpret_cast<const uint32_t*>(src));
       }
-#pragma unroll
-      for (int i = 0; i < E / 2; ++i) {
-        if (a.bf16) {
-          x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        } else {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-          x[2 * i] = f.x, x[2 * i + 1] = f.y;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < E; ++i) x[i] = 0.0f;
-    }
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < E; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-    top = __reduce_max_sync(0xffffffffu, top);
-    float up, down;
-    row_factor(__uint_as_float(top), up, down);
-#pragma unroll
-    for (int i = 0; i < E / 2; ++i)
-      *reinterpret_cast<uint32_t*>(&s_q[r * kQStride + lane * E + 2 * i]) = pack_half2(x[2 * i] * up, x[2 * i + 1] * up);
-    if (lane == 0) {
-      const int p = len - T + row / a.group;
-      s_down[r] = down;
-      s_hi[r] = live ? (a.causal ? min(len, p + 1) : len) : 0;
-      s_lo[r] = a.window ? p - a.window + 1 : 0;
     }
   }
-  __syncthreads();
 
   float acc[NT][MT][4], m[NT][2], l[NT][2], f[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) m[n][i] = -INFINITY, l[n][i] = 0.0f, f[n][i] = s_down[8 * n + 2 * q4 + i];
+    for (int i = 0; i < 2; ++i) m[n][i] = -INFINITY, l[n][i] = 0.0f;
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -179,12 +153,8 @@ __global__ void __launch_bounds__(kWarps * 32)
   for (long long seg0 = keys.lo; seg0 < keys.hi; seg0 += seg_keys) {
     const int seg = static_cast<int>(seg0), seg_hi = static_cast<int>(min(static_cast<long long>(keys.hi), seg0 + seg_keys));
     const int blk0 = seg >> bs_log2, nblk = ((seg_hi - 1) >> bs_log2) - blk0 + 1;
-    for (int i = threadIdx.x; i < nblk; i += kWarps * 32) {
-      const long long id = block_of(a.seqs, a.pages, b, blk0 + i);
-      s_id[i] = static_cast<int>(id);
-      const BlockScales s = fold_scales(a, raw_scales(a, id, h));
-      s_c[i] = s.c, s_lw[i] = s.log2_w, s_iw[i] = s.inv_w;
-    }
+    for (int i = threadIdx.x; i < nblk; i += kWarps * 32)
+      s_id[i] = static_cast<int>(block_of(a.seqs, a.pages, b, blk0 + i));
     __syncthreads();
 
     const int groups = (seg_hi - seg + 15) >> 4, tiles = (groups + K16 - 1) / K16;
@@ -208,6 +178,47 @@ __global__ void __launch_bounds__(kWarps * 32)
     const uint32_t turn0 = turn;
     for (int i = 0; i < Rg::stages; ++i)
       if (warp + i * kWarps < tiles) copy(warp + i * kWarps, turn0 + i);
+
+    if (seg0 == keys.lo) {  // the rows of q, each scaled by a power of two into f16
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int r = warp + i * kWarps, row = r0 + r;
+        float x[E];
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) {
+          if (a.bf16) {
+            x[2 * e] = __uint_as_float(qw[i][e] << 16), x[2 * e + 1] = __uint_as_float(qw[i][e] & 0xffff0000u);
+          } else {
+            const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&qw[i][e]));
+            x[2 * e] = v.x, x[2 * e + 1] = v.y;
+          }
+        }
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+        top = __reduce_max_sync(0xffffffffu, top);
+        float up, down;
+        row_factor(__uint_as_float(top), up, down);
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e)
+          *reinterpret_cast<uint32_t*>(&s_q[r * kQStride + lane * E + 2 * e]) = pack_half2(x[2 * e] * up, x[2 * e + 1] * up);
+        if (lane == 0) {
+          const int p = len - T + row / a.group;
+          s_down[r] = down;
+          s_hi[r] = row < r1 ? (a.causal ? min(len, p + 1) : len) : 0;
+          s_lo[r] = a.window ? p - a.window + 1 : 0;
+        }
+      }
+    }
+    for (int i = threadIdx.x; i < nblk; i += kWarps * 32) {
+      const BlockScales s = fold_scales(a, raw_scales(a, s_id[i], h));
+      s_c[i] = s.c, s_lw[i] = s.log2_w, s_iw[i] = s.inv_w;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) f[n][i] = s_down[8 * n + 2 * q4 + i];
     for (int tile = warp; tile < tiles && ok; tile += kWarps, ++turn) {
       ok = warp_wait(&s_full[warp][turn % Rg::stages], (turn / Rg::stages) & 1, err, kErrTimeoutFull);
       if (!ok) break;
@@ -359,7 +370,9 @@ __global__ void __launch_bounds__(kWarps * 32)
     if (!__syncthreads_and(ok)) break;
   }
 
-  // join the warps: every row's maximum, then the rows added up one warp after the other
+  griddep_launch_dependents();
+  // join the warps: every row's maximum, then the warps' rows beside one another in the rings' memory, or on top of
+  // one another where they do not fit
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -369,8 +382,9 @@ __global__ void __launch_bounds__(kWarps * 32)
       if (g == 0) s_m[warp][8 * n + 2 * q4 + i] = m[n][i], s_l[warp][8 * n + 2 * q4 + i] = l[n][i];
     }
   __syncthreads();
-  for (int w = 0; w < kWarps; ++w) {
-    if (warp == w) {
+  constexpr int kArea = kRows * kOStride, kAreas = kWarps * kArea * 4 <= Rg::smem - 1024 ? kWarps : kWarps / 2;
+  for (int w = 0; w < kWarps; w += kAreas) {
+    if (warp >= w && warp < w + kAreas) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -380,13 +394,14 @@ __global__ void __launch_bounds__(kWarps * 32)
 #pragma unroll
           for (int x = 1; x < kWarps; ++x) top = fmaxf(top, s_m[x][r]);
           const float alpha = ex2(m[n][i] - (top == -INFINITY ? 0.0f : top));
-          float* o = s_o + r * kOStride;
+          float* o = s_o + (warp - w) * kArea + r * kOStride;
 #pragma unroll
           for (int t = 0; t < MT; ++t) {
-            const float x0 = acc[n][t][i] * alpha, x1 = acc[n][t][i + 2] * alpha;
             const int d = D == 64 ? 8 * g + 2 * t : 128 * (t >> 3) + 16 * g + 2 * (t & 7);
-            o[d] = w ? o[d] + x0 : x0;
-            o[d + 1] = w ? o[d + 1] + x1 : x1;
+            float2 x = make_float2(acc[n][t][i] * alpha, acc[n][t][i + 2] * alpha);
+            float2* to = reinterpret_cast<float2*>(o + d);
+            if (w) x.x += to->x, x.y += to->y;
+            *to = x;
           }
         }
     }
@@ -406,7 +421,11 @@ __global__ void __launch_bounds__(kWarps * 32)
     for (int w = 0; w < kWarps; ++w) sum += s_l[w][r] * ex2(s_m[w][r] - base);
     float o[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = s_o[r * kOStride + 8 * c + e];
+    for (int e = 0; e < 8; ++e) {
+      o[e] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kAreas; ++w) o[e] += s_o[w * kArea + r * kOStride + 8 * c + e];
+    }
     if (a.chunks == 1) {
       write_row8(a, b, row0, row, h, 8 * c, o, sum, base);
     } else {
