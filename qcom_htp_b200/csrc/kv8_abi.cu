@@ -133,7 +133,7 @@ QhtpStatus plan_attention(const QhtpKv8Attention* run, Kv8Attn* a) {
     kv8_decode_plan(*a, sm_count());
   if (a->prompt && a->row_groups > 65535) return unsupported("kv8: too many rows");
   if (static_cast<long long>(a->chunks) * a->pages.heads > (1ll << 30)) return unsupported("kv8: too many chunks");
-  if (static_cast<long long>(a->chunks) * a->row_groups > (1ll << 30)) return unsupported("kv8: too many rows");
+  if (static_cast<long long>(a->pages.heads) * a->row_groups > (1ll << 30)) return unsupported("kv8: too many rows");
   return QHTP_STATUS_OK;
 }
 

@@ -69,7 +69,7 @@ struct Ring {
 };
 
 template <int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 3)  // as many as the rings leave room for
     kv8_decode_kernel(const Kv8Attn a, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
   using Rg = Ring<D, NT>;
   constexpr int K16 = Rg::k16;
@@ -90,7 +90,8 @@ __global__ void __launch_bounds__(kWarps * 32)
   float* const s_o = reinterpret_cast<float*>(ring);
   int* const err = &g_error;
 
-  const int b = blockIdx.z, h = blockIdx.y, rg = blockIdx.x / a.chunks, chunk = blockIdx.x - rg * a.chunks;
+  // chunks slowest: the first ones, which every sequence has whole, run first, and the remainders fill the end
+  const int b = blockIdx.y, h = blockIdx.x / a.row_groups, rg = blockIdx.x - h * a.row_groups, chunk = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
   long long row0;
   const int T = seq_rows(a.seqs, b, row0);
@@ -566,7 +567,7 @@ cudaError_t run(const Kv8Attn& a) {
   const cudaError_t e =
       cudaFuncSetAttribute(kv8_decode_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Rg::smem);
   if (e != cudaSuccess) return e;
-  const dim3 grid(static_cast<unsigned>(a.chunks) * a.row_groups, a.pages.heads, a.seqs.batch);
+  const dim3 grid(static_cast<unsigned>(a.pages.heads) * a.row_groups, a.seqs.batch, a.chunks);
   kv8_decode_kernel<D, NT><<<grid, kWarps * 32, Rg::smem, a.stream>>>(a, map[0], map[1]);
   return cudaGetLastError();
 }
@@ -612,6 +613,7 @@ void kv8_decode_plan(Kv8Attn& a, int sms) {
     n = (span + kMost - 1) / kMost;
     if (n * tiles < 4 * slots) n = std::max(1ll, std::min(slots / tiles, span / kLeast));
   }
+  n = std::min(n, 65535ll);  // grid.z
   const long long chunk = ((span + n - 1) / n + 127) / 128 * 128;
   a.chunk = static_cast<int>(chunk);
   a.chunks = static_cast<int>((span + chunk - 1) / chunk);
