@@ -17,8 +17,8 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libqhtp.so"
 SOURCES = ["qhtp_abi.cu", "qgemm.cu", "qdecode.cu", "gdn.cu", "gdn256.cu", "gdn256x2.cu", "noalloc.cu", "wire.cu", "gdn256f.cu", "qgroup.cu", "peak.cu", "qchain.cu", "qdec4.cu",
-           "kv8_abi.cu", "kv8_cache.cu", "kv8_decode.cu", "kv8_prompt.cu"]
-HEADERS = ["ptx.cuh", "requant.cuh", "internal.h", "gdn_common.cuh", "kv8.cuh"]
+           "kv8_abi.cu", "kv8_cache.cu", "kv8_decode.cu", "kv8_prompt.cu", "kv8_prompt2.cu"]
+HEADERS = ["ptx.cuh", "requant.cuh", "internal.h", "gdn_common.cuh", "kv8.cuh", "kv8_prompt.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

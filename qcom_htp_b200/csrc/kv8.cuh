@@ -262,11 +262,14 @@ cudaError_t launch_kv8_decode(const Kv8Attn& a);
 // kv8_prompt.cu: rows in tiles of 128 or 256 on tcgen05
 void kv8_prompt_plan(Kv8Attn& a, int sms);
 cudaError_t launch_kv8_prompt(const Kv8Attn& a);
+// kv8_prompt2.cu: tiles of 256 rows, head_dim 64 and 128
+cudaError_t launch_kv8_prompt2(const Kv8Attn& a);
 
 // joins the chunks of a launch
 cudaError_t launch_kv8_combine(const Kv8Attn& a);
 // the current device's error words of the two (a wait that gave up leaves its code), read and cleared; synchronizes
 cudaError_t kv8_prompt_error(int* code, cudaStream_t stream);
+cudaError_t kv8_prompt2_error(int* code, cudaStream_t stream);
 cudaError_t kv8_decode_error(int* code, cudaStream_t stream);
 inline cudaError_t kv8_take_error(const void* symbol, int* code, cudaStream_t stream) {
   void* at = nullptr;

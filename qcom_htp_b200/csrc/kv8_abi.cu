@@ -176,18 +176,19 @@ QhtpStatus qhtp_kv8_attention(const QhtpKv8Attention* run) {
   a.lse = run->lse;
   a.part = static_cast<float*>(run->workspace);
   a.stream = static_cast<cudaStream_t>(run->stream);
-  cudaError_t e = a.prompt ? launch_kv8_prompt(a) : launch_kv8_decode(a);
+  cudaError_t e = a.prompt ? (a.tile_rows == 256 ? launch_kv8_prompt2(a) : launch_kv8_prompt(a)) : launch_kv8_decode(a);
   if (e == cudaSuccess && a.chunks > 1) e = launch_kv8_combine(a);
   return status_from_cuda(e);
 }
 
 QhtpStatus qhtp_kv8_check(int* device_code, void* stream) {
-  int code = 0, other = 0;
-  cudaError_t e = kv8_prompt_error(&code, static_cast<cudaStream_t>(stream));
-  if (e == cudaSuccess) e = kv8_decode_error(&other, static_cast<cudaStream_t>(stream));
-  const QhtpStatus st = status_from_cuda(e);
-  if (st != QHTP_STATUS_OK) return st;
-  if (code == 0) code = other;
+  int code = 0;
+  for (auto read : {kv8_decode_error, kv8_prompt_error, kv8_prompt2_error}) {
+    int one = 0;
+    const QhtpStatus st = status_from_cuda(read(&one, static_cast<cudaStream_t>(stream)));
+    if (st != QHTP_STATUS_OK) return st;
+    if (code == 0) code = one;
+  }
   if (device_code != nullptr) *device_code = code;
   if (code == 0) return QHTP_STATUS_OK;
   set_last_message("kv8: a wait inside an attention kernel gave up");

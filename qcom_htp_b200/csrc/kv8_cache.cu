@@ -13,7 +13,11 @@
 // written by that CTA alone: no atomics, and the same bytes in every run.
 //
 // Bound by memory: per element the input is read once (2 or 4 bytes) and one code byte is written; a
-// tile's rows stay in registers between the maximum and the rounding.
+// tile's rows stay in registers between the maximum and the rounding.  Conversions between integers and floats run at a
+// quarter of the rate of additions and took longer than the memory here, so both directions go through additions:
+// y + 1.5 2^23 leaves rint(y) in its low bits, and 2^23 + (code + 128) is made by placing a byte.
+#include <type_traits>
+
 #include "kv8.cuh"
 
 namespace qhtp {
@@ -30,10 +34,41 @@ struct MoveArgs {
   int vec_log2;  // 16-byte vectors of a row
 };
 
+// rint of two's-complement bytes: the low byte of y + 1.5 2^23, |y| < 2^22 (y here is at most 127 and a rounding).
+__device__ __forceinline__ uint32_t round_bits(float y) { return __float_as_uint(__fadd_rn(y, 12582912.0f)); }
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return prmt(prmt(a, b, 0x0040u), prmt(c, d, 0x0040u), 0x5410u);
+}
+// Four int8 codes -> float32, exactly.
+__device__ __forceinline__ void codes_to_float(uint32_t w, float (&f)[4]) {
+  w ^= 0x80808080u;
+  f[0] = __uint_as_float(prmt(w, 0x4b000000u, 0x7440u)) - 8388736.0f;
+  f[1] = __uint_as_float(prmt(w, 0x4b000000u, 0x7441u)) - 8388736.0f;
+  f[2] = __uint_as_float(prmt(w, 0x4b000000u, 0x7442u)) - 8388736.0f;
+  f[3] = __uint_as_float(prmt(w, 0x4b000000u, 0x7443u)) - 8388736.0f;
+}
+// The largest |x| of 16 bytes of T, as the bits of T (for the 16-bit types of both halves of the word): magnitudes are
+// ordered like their bits, infinity and NaN above all others.
+template <typename T>
+__device__ __forceinline__ uint32_t max_bits(uint32_t top, const uint4& r) {
+  if constexpr (Vec<T>::n == 4)
+    return max(max(max(top, r.x & 0x7fffffffu), r.y & 0x7fffffffu), max(r.z & 0x7fffffffu, r.w & 0x7fffffffu));
+  else
+    return __vmaxu2(__vmaxu2(__vmaxu2(top, r.x & 0x7fff7fffu), r.y & 0x7fff7fffu),
+                    __vmaxu2(r.z & 0x7fff7fffu, r.w & 0x7fff7fffu));
+}
+template <typename T>
+__device__ __forceinline__ float max_value(uint32_t top) {
+  if constexpr (Vec<T>::n == 4) return __uint_as_float(top);
+  top = max(top & 0xffffu, top >> 16);
+  if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half(static_cast<unsigned short>(top)));
+  return __uint_as_float(top << 16);
+}
+
 // One CTA per (block of the sequence, K or V of a head, sequence).  NV: vectors a thread keeps in
 // registers; tiles with more than NV per thread read their rows a second time (from L2).
 template <typename T, int NV>
-__global__ void __launch_bounds__(kMaxThreads) kv8_write_kernel(const MoveArgs a) {
+__global__ void __launch_bounds__(kMaxThreads, NV <= 4 ? 6 : 3) kv8_write_kernel(const MoveArgs a) {
   constexpr int VN = Vec<T>::n;
   const int b = blockIdx.z, h = blockIdx.y >> 1, kv = blockIdx.y & 1;
   long long row0;
@@ -61,21 +96,16 @@ __global__ void __launch_bounds__(kMaxThreads) kv8_write_kernel(const MoveArgs a
     return __ldg(reinterpret_cast<const uint4*>(x + (i >> a.vec_log2) * src.token_stride + (i & cmask) * VN));
   };
   uint4 raw[NV];
-  uint32_t top = 0;  // max |x| as bits: ordered like the values, infinity and NaN above all of them
-  auto take = [&](const uint4& r) {
-    float f[VN];
-    Vec<T>::load(r, f);
-#pragma unroll
-    for (int e = 0; e < VN; ++e) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
-  };
+  uint32_t bits = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int at = threadIdx.x + i * blockDim.x;
     raw[i] = at < nvec ? load(at) : make_uint4(0, 0, 0, 0);
   }
 #pragma unroll
-  for (int i = 0; i < NV; ++i) take(raw[i]);
-  for (int at = threadIdx.x + NV * blockDim.x; at < nvec; at += blockDim.x) take(load(at));
+  for (int i = 0; i < NV; ++i) bits = max_bits<T>(bits, raw[i]);
+  for (int at = threadIdx.x + NV * blockDim.x; at < nvec; at += blockDim.x) bits = max_bits<T>(bits, load(at));
+  uint32_t top = __float_as_uint(max_value<T>(bits));
 
   __shared__ uint32_t s_top[kMaxThreads / 32];
   top = __reduce_max_sync(0xffffffffu, top);
@@ -95,16 +125,12 @@ __global__ void __launch_bounds__(kMaxThreads) kv8_write_kernel(const MoveArgs a
     float f[VN];
     Vec<T>::load(r, f);
     uint32_t w[VN / 4];
+    // no |x| is above the s it was divided by, so no code is above 127
 #pragma unroll
     for (int e = 0; e < VN / 4; ++e) {
-      uint32_t c[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        // with inv 0 a NaN or infinity gives NaN here; fminf / fmaxf then return a bound
-        const float q = fminf(fmaxf(rintf(__fmul_rn(f[4 * e + j], inv)), -127.0f), 127.0f);
-        c[j] = fine ? static_cast<uint32_t>(__float2int_rn(q)) : 0u;
-      }
-      w[e] = prmt(prmt(c[0], c[1], 0x0040u), prmt(c[2], c[3], 0x0040u), 0x5410u);
+      const uint32_t c = low_bytes(round_bits(__fmul_rn(f[4 * e], inv)), round_bits(__fmul_rn(f[4 * e + 1], inv)),
+                                   round_bits(__fmul_rn(f[4 * e + 2], inv)), round_bits(__fmul_rn(f[4 * e + 3], inv)));
+      w[e] = fine ? c : 0u;
     }
     int8_t* to = codes + ((slot0 << a.vec_log2) + at) * VN;
     if constexpr (VN == 8)
@@ -129,21 +155,26 @@ __global__ void __launch_bounds__(kMaxThreads) kv8_write_kernel(const MoveArgs a
     uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      uint32_t c[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        c[j] = static_cast<uint32_t>(
-            __float2int_rn(__fmul_rn(static_cast<float>(static_cast<int8_t>(w[e] >> (8 * j))), ratio)));
-      w[e] = prmt(prmt(c[0], c[1], 0x0040u), prmt(c[2], c[3], 0x0040u), 0x5410u);
+      float f[4];
+      codes_to_float(w[e], f);
+      w[e] = low_bytes(round_bits(__fmul_rn(f[0], ratio)), round_bits(__fmul_rn(f[1], ratio)),
+                       round_bits(__fmul_rn(f[2], ratio)), round_bits(__fmul_rn(f[3], ratio)));
     }
     held[i] = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
-// One CTA per (block of the sequence, K or V of a head, sequence), 16 codes a thread and step.  Rows whose block the table does not map come back as NaN.
+// Codes that a reading thread takes at a time: 16 for 16-bit rows (two 16-byte stores, a whole sector), 4 for float32.
+template <typename T>
+constexpr int codes_of() {
+  return Vec<T>::n == 8 ? 16 : 4;
+}
+
+// One CTA per (block of the sequence, K or V of a head, sequence).
+// Rows whose block the table does not map come back as NaN.
 template <typename T>
 __global__ void __launch_bounds__(kMaxThreads) kv8_read_kernel(const MoveArgs a) {
-  constexpr int VN = Vec<T>::n;
+  constexpr int VN = Vec<T>::n, kCodes = codes_of<T>();
   const int b = blockIdx.z, h = blockIdx.y >> 1, kv = blockIdx.y & 1;
   long long row0;
   const int n = seq_rows(a.seqs, b, row0);
@@ -154,7 +185,7 @@ __global__ void __launch_bounds__(kMaxThreads) kv8_read_kernel(const MoveArgs a)
   if (lo >= hi) return;
   const long long id = block_of(a.seqs, a.pages, b, blk);
   const int slot0 = static_cast<int>(lo - (blk << bs_log2)), rows = static_cast<int>(hi - lo);
-  const int d = 16 << a.vec_log2;
+  const int d = kCodes << a.vec_log2;
   const long long tile = max(id, 0ll) * a.pages.heads + h;
   const int8_t* codes = (kv ? a.pages.v : a.pages.k) + ((tile << bs_log2) + slot0) * d;
   const float s = id < 0 ? nan_f32() : (kv ? a.pages.v_scale : a.pages.k_scale)[tile];
@@ -163,16 +194,23 @@ __global__ void __launch_bounds__(kMaxThreads) kv8_read_kernel(const MoveArgs a)
   const int nvec = rows << a.vec_log2, cmask = (1 << a.vec_log2) - 1;
 #pragma unroll 4
   for (int i = threadIdx.x; i < nvec; i += blockDim.x) {
-    const uint4 r = __ldg(reinterpret_cast<const uint4*>(codes) + i);
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-    T* to = x + (i >> a.vec_log2) * dst.token_stride + (i & cmask) * 16;
+    uint32_t w[kCodes / 4];
+    if constexpr (kCodes == 16) {
+      const uint4 r = __ldg(reinterpret_cast<const uint4*>(codes) + i);
+      w[0] = r.x, w[1] = r.y, w[2] = r.z, w[3] = r.w;
+    } else {
+      w[0] = __ldg(reinterpret_cast<const uint32_t*>(codes) + i);
+    }
+    T* const to = x + (i >> a.vec_log2) * dst.token_stride + (i & cmask) * kCodes;
 #pragma unroll
-    for (int e = 0; e < 16 / VN; ++e) {
+    for (int e = 0; e < kCodes / VN; ++e) {
       float f[VN];
 #pragma unroll
-      for (int j = 0; j < VN; ++j) {
-        const int at = e * VN + j;
-        f[j] = __fmul_rn(static_cast<float>(static_cast<int8_t>(w[at >> 2] >> (8 * (at & 3)))), s);
+      for (int j = 0; j < VN / 4; ++j) {
+        float g[4];
+        codes_to_float(w[e * VN / 4 + j], g);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f[4 * j + k] = __fmul_rn(g[k], s);
       }
       *reinterpret_cast<uint4*>(to + e * VN) = Vec<T>::store(f);
     }
@@ -212,10 +250,11 @@ cudaError_t write(const Kv8Move& m) {
 
 template <typename T>
 cudaError_t read(const Kv8Move& m) {
-  MoveArgs a{m.pages, m.seqs, m.first, {m.k, m.v}, log2_of(m.head_dim / 16)};
+  constexpr int kCodes = codes_of<T>();
+  MoveArgs a{m.pages, m.seqs, m.first, {m.k, m.v}, log2_of(m.head_dim / kCodes)};
   const dim3 grid(blocks_touched(m), 2 * m.pages.heads, m.seqs.batch);
   const int rows = m.seqs.tokens < (1 << m.pages.bs_log2) ? m.seqs.tokens : 1 << m.pages.bs_log2;
-  const int vecs = rows * m.head_dim / 16;
+  const int vecs = rows * m.head_dim / kCodes;
   kv8_read_kernel<T><<<grid, vecs >= 512 ? 256 : 128, 0, m.stream>>>(a);
   return cudaGetLastError();
 }
