@@ -27,7 +27,7 @@ struct Shape2 {
   static constexpr int smem = 2 * q_tile + 4 * tile + kStaged * staging + 1024;
   static constexpr int threads = 768;
   // registers of a thread: at launch, and by role (four softmax warpgroups, one of converters, one with the issuing warp)
-  static constexpr int regs = 80, softmax_regs = 96, convert_regs = 56, mma_regs = 40;
+  static constexpr int regs = 80, softmax_regs = 96, convert_regs = 48, mma_regs = 48;
   static_assert(4 * softmax_regs + convert_regs + mma_regs <= 6 * regs, "registers");
   // tensor memory columns: S of the two tiles, O of the two, Q of the two where there is room
   static constexpr bool q_tmem = D == 64;
@@ -35,7 +35,7 @@ struct Shape2 {
 };
 
 struct Barriers2 {
-  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], drained, staged[kStaged];
+  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], drained, staged[kStaged], taken[kStaged];
 };
 
 __device__ int g_error2;  // a wait that gave up leaves its code here
@@ -72,21 +72,21 @@ __global__ void __launch_bounds__(Shape2<D>::threads, 1) kv8_prompt2_kernel(cons
   uint8_t* const v_img = k_img + 2 * S::tile;
   uint8_t* const stage_img = v_img + 2 * S::tile;
 
-  constexpr int kConv = 16, kMma = 20;  // first warps of the roles
+  constexpr int kConv = 16, kMma = 20, kCopy = 21, kScale = 22;  // first warps of the roles
   if (warp == kMma) {
     tmem_alloc(&s_tmem, 512);
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) {
         mbar_init(&bar.q_full[i], 256);
-        mbar_init(&bar.k_full[i], 128);
-        mbar_init(&bar.v_full[i], 128);
+        mbar_init(&bar.k_full[i], 5);  // the converter warps, and the one that brings the scales
+        mbar_init(&bar.v_full[i], 4);
         mbar_init(&bar.k_empty[i], 1);
         mbar_init(&bar.v_empty[i], 1);
         mbar_init(&bar.s_full[i], 2);  // the MMAs, and the issuing thread's own arrival
         mbar_init(&bar.p_full[i], 256);
         mbar_init(&bar.o_full[i], 1);
       }
-      for (int i = 0; i < kStaged; ++i) mbar_init(&bar.staged[i], 1);
+      for (int i = 0; i < kStaged; ++i) mbar_init(&bar.staged[i], 1), mbar_init(&bar.taken[i], 4);
       mbar_init(&bar.drained, 1);
       fence_barrier_init();
     }
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(Shape2<D>::threads, 1) kv8_prompt2_kernel(cons
   } else if (warp < kMma) {
     // ------------------------------------------------------------------------------- codes to f16 images
     reg_free<S::convert_regs>();
-    // Pieces in the order of their use: K's two units of a tile, V's two, the next tile's.
+    // Pieces of 64 keys in the order of their use: K's two of a tile, V's two, the next tile's.
     constexpr int kStep = 128 / (D / 8), kSteps = kUnit / kStep;
     const int t = threadIdx.x - kConv * 32;
     // A thread has chunk c (eight codes, 16 bytes as f16) of the rows row, row + kStep, ...: loads and stores of a
@@ -250,85 +250,79 @@ __global__ void __launch_bounds__(Shape2<D>::threads, 1) kv8_prompt2_kernel(cons
     const int c = t % (D / 8), row = t / (D / 8);
     const uint32_t from = smem_u32(stage_img) + row * D + c * 8;
     const uint32_t to = smem_u32(k_img) + (c >> 3) * kPanel2 + swizzled(row, c & 7);
-    const bool first_warp = warp == kConv;  // brings the codes and the scales
-    const int bs_log2 = a.pages.bs_log2, bs = 1 << bs_log2, pieces = 4 * tiles;
+    bool ok = true;
+    for (int n = 0; n < 4 * tiles && ok; ++n) {
+      const int j = n >> 2, q = n & 3, st = j & 1, at = n % kStaged;
+      if (!warp_wait(&bar.staged[at], (n / kStaged) & 1, err, kErrTimeoutFull)) break;
+      uint2 raw[kSteps];
+#pragma unroll
+      for (int e = 0; e < kSteps; ++e) raw[e] = lds64(from + at * S::staging + e * kStep * D);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar.taken[at]);
+      if ((q & 1) == 0 && j >= 2)
+        ok = warp_wait(q ? &bar.v_empty[st] : &bar.k_empty[st], ((j >> 1) - 1) & 1, err, kErrTimeoutEmpty);
+      const uint32_t img = to + (q & 2 ? 2 * S::tile : 0) + st * S::tile + (q & 1) * (kUnit * 128);
+#pragma unroll
+      for (int e = 0; e < kSteps; ++e) {
+        uint32_t u[4];
+        codes_to_half2(raw[e].x, u[0], u[1]);
+        codes_to_half2(raw[e].y, u[2], u[3]);
+        sts128(img + e * kStep * 128, u[0], u[1], u[2], u[3]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if ((q & 1) && lane == 0) mbar_arrive(q & 2 ? &bar.v_full[st] : &bar.k_full[st]);
+    }
+  } else {
+    // ------------------------------------------------------------------------------- the MMAs
+    reg_free<S::mma_regs>();
+    const int bs_log2 = a.pages.bs_log2, bs = 1 << bs_log2;
     // block of the tile's 16-key group `lane` (of eight); -1: none
     auto ids_of = [&](int j) {
       const int key = keys.lo + j * kTile + 16 * (lane & 7);
       return j < tiles && key < keys.hi ? static_cast<int>(block_of(a.seqs, a.pages, b, key >> bs_log2)) : -1;
     };
-    // groups that there are none of keep the codes that happen to be there: they are hidden, or their scales are NaN
-    auto copy = [&](int n, int id) {
-      const int j = n >> 2, u = n & 1, at = n % kStaged;
-      const bool there = (lane >> 2) == u && id >= 0;
-      const int count = __popc(__ballot_sync(0xffffffffu, there));
-      if (lane == 0) mbar_arrive_expect_tx(&bar.staged[at], count * 16 * D);
-      __syncwarp();
-      if (there) {
-        const int slot = (keys.lo + j * kTile + 16 * lane) & (bs - 1);
-        bulk_load(stage_img + at * S::staging + (lane & 3) * 16 * D,
-                  (n & 2 ? a.pages.v : a.pages.k) + (((static_cast<long long>(id) * a.pages.heads + h) << bs_log2) + slot) * D,
-                  16 * D, &bar.staged[at]);
-      }
-    };
-    // blocks of this tile and the next (only the first warp's are used)
-    int id = ids_of(0), id_next = ids_of(1), issued = 0;
-    RawScales sc{};
-    if (first_warp && tiles > 0) {
-      for (; issued < kStaged; ++issued) copy(issued, id);
-      sc = raw_scales(a, id, h);
-    }
-    bool ok = true;
-    for (int j = 0; j < tiles; ++j) {
-      const int st = j & 1;
-      const uint32_t again = ((j >> 1) - 1) & 1;
-      RawScales sc_next{};
-      int id_after = -1;
-      if (first_warp) {
-        sc_next = raw_scales(a, id_next, h);
-        id_after = ids_of(j + 2);
-      }
-#pragma unroll 1
-      for (int q = 0; q < 4; ++q) {
-        const int n = 4 * j + q, at = n % kStaged;
-        // after a wait that gave up nothing is brought or waited for, but every warp still passes every named barrier
-        ok = ok && warp_wait(&bar.staged[at], (n / kStaged) & 1, err, kErrTimeoutFull);
-        uint2 raw[kSteps];
-#pragma unroll
-        for (int e = 0; e < kSteps; ++e) raw[e] = lds64(from + at * S::staging + e * kStep * D);
-        named_barrier(3, 128);  // the staging buffer is read
-        if (ok && first_warp && n + kStaged < pieces) {
-          copy(n + kStaged, (n + kStaged) >> 2 == j ? id : id_next);
-          ++issued;
+    if (warp == kCopy) {
+      // codes to the staging buffers, in the order of their use; the table's entries are read a tile ahead.  Groups that there
+      // are none of keep the codes that happen to be there: they are hidden, or their scales are NaN.
+      int id = -1, id_next = ids_of(0), n = 0;
+      bool ok = true;
+      for (; n < 4 * tiles; ++n) {
+        const int j = n >> 2, u = n & 1, at = n % kStaged;
+        if ((n & 3) == 0) id = id_next, id_next = ids_of(j + 1);
+        if (n >= kStaged) ok = warp_wait(&bar.taken[at], ((n / kStaged) - 1) & 1, err, kErrTimeoutEmpty);
+        if (!ok) break;
+        const bool there = (lane >> 2) == u && id >= 0;
+        const int count = __popc(__ballot_sync(0xffffffffu, there));
+        if (lane == 0) mbar_arrive_expect_tx(&bar.staged[at], count * 16 * D);
+        __syncwarp();
+        if (there) {
+          const int slot = (keys.lo + j * kTile + 16 * lane) & (bs - 1);
+          bulk_load(stage_img + at * S::staging + (lane & 3) * 16 * D,
+                    (n & 2 ? a.pages.v : a.pages.k) + (((static_cast<long long>(id) * a.pages.heads + h) << bs_log2) + slot) * D,
+                    16 * D, &bar.staged[at]);
         }
-        if ((q & 1) == 0 && j >= 2) ok = ok && warp_wait(q ? &bar.v_empty[st] : &bar.k_empty[st], again, err, kErrTimeoutEmpty);
-        if (q == 0 && first_warp) {
-          // .w: a group whose scales need care (zero, or not finite)
-          const BlockScales f = fold_scales(a, sc);
-          const bool odd = !(f.inv_w < kZeroTile) || !isfinite(f.c);
-          const float care = __any_sync(0xffffffffu, odd) ? 1.0f : 0.0f;
-          if (lane < 8) s_scale[j & 3][lane] = make_float4(f.c, f.log2_w, f.inv_w, care);
-        }
-        const uint32_t img = to + (q & 2 ? 2 * S::tile : 0) + st * S::tile + (q & 1) * (kUnit * 128);
-#pragma unroll
-        for (int e = 0; e < kSteps; ++e) {
-          uint32_t u[4];
-          codes_to_half2(raw[e].x, u[0], u[1]);
-          codes_to_half2(raw[e].y, u[2], u[3]);
-          sts128(img + e * kStep * 128, u[0], u[1], u[2], u[3]);
-        }
-        fence_proxy_async_smem();
-        if (q & 1) mbar_arrive(q & 2 ? &bar.v_full[st] : &bar.k_full[st]);
       }
-      id = id_next, id_next = id_after, sc = sc_next;
-    }
-    if (!ok && first_warp)  // a wait gave up: copies under way end before the block does
-      for (int n = std::max(0, issued - kStaged); n < issued; ++n)
-        warp_wait(&bar.staged[n % kStaged], (n / kStaged) & 1, err, kErrTimeoutOther);
-  } else {
-    // ------------------------------------------------------------------------------- the MMAs
-    reg_free<S::mma_regs>();
-    if (warp == kMma && tiles > 0) {
+      if (!ok)  // copies under way end before the block does
+        for (int i = max(0, n - kStaged); i < n; ++i)
+          warp_wait(&bar.staged[i % kStaged], (i / kStaged) & 1, err, kErrTimeoutOther);
+    } else if (warp == kScale) {
+      int id_next = ids_of(1);
+      RawScales sc = tiles > 0 ? raw_scales(a, ids_of(0), h) : RawScales{};
+      for (int j = 0; j < tiles; ++j) {
+        const RawScales next = raw_scales(a, id_next, h);
+        id_next = ids_of(j + 2);
+        if (j >= 2 && !warp_wait(&bar.k_empty[j & 1], ((j >> 1) - 1) & 1, err, kErrTimeoutEmpty)) break;
+        // .w: a group whose scales need care (zero, or not finite)
+        const BlockScales f = fold_scales(a, sc);
+        const bool odd = !(f.inv_w < kZeroTile) || !isfinite(f.c);
+        const float care = __any_sync(0xffffffffu, odd) ? 1.0f : 0.0f;
+        if (lane < 8) s_scale[j & 3][lane] = make_float4(f.c, f.log2_w, f.inv_w, care);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.k_full[j & 1]);
+        sc = next;
+      }
+    } else if (warp == kMma && tiles > 0) {
       const int slots = r0 + 128 < r1 ? 2 : 1;
       constexpr uint32_t id_qk = idesc_f16(128, kTile), id_pv = idesc_f16(128, D, 1);
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), leader = elect_one();
