@@ -202,42 +202,15 @@ __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const 
     // the rows
     const float base = m == -INFINITY ? 0.0f : m;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const long long part0 = part_row(a, b, h, rg, chunk) + warp * 32, part = part0 + lane;
+    // K's images are free: every S has been computed
+    rows_out<D, D>(a, b, h, row0, r0 + warp * 32, r1, part0, units == 0, o_at, 0, inv, smem_u32(k_img) + warp * 4096, lane);
     const bool live = r < r1;
-    const int t = r / a.group, head = h * a.group + r - t * a.group;
-    const long long part = part_row(a, b, h, rg, chunk) + in_tile;
-    uint16_t* out = static_cast<uint16_t*>(a.out.data) + b * a.out.batch_stride + (row0 + t) * a.out.token_stride +
-                    head * a.out.head_stride;
-#pragma unroll 1
-    for (int c = 0; c < D / 32; ++c) {
-      uint32_t x[32];
-      if (units > 0) {
-        tmem_ld32(o_at + 32 * c, x);
-        tmem_ld_wait();
-        pin(x);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 32; ++e) x[e] = 0;
-      }
-      __syncwarp();
-      if (live && a.chunks == 1) {
-#pragma unroll
-        for (int e = 0; e < 32; e += 8) {
-          float v[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(x[e + i]) * inv;
-          *reinterpret_cast<uint4*>(out + 32 * c + e) = a.bf16 ? Vec<__nv_bfloat16>::store(v) : Vec<__half>::store(v);
-        }
-      } else if (live) {
-        uint4* to = reinterpret_cast<uint4*>(a.part + part * D + 32 * c);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) to[e] = make_uint4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
-      }
-      __syncwarp();
-    }
     if (live && a.chunks > 1) {
       float* ml = a.part + part_rows(a) * D + 2 * part;
       ml[0] = base, ml[1] = l;
     } else if (live && a.lse != nullptr) {
+      const int t = r / a.group, head = h * a.group + r - t * a.group;
       const long long at = (a.seqs.start ? row0 : static_cast<long long>(b) * a.seqs.tokens) + t;
       a.lse[at * a.q_heads + head] = l == 0.0f ? -INFINITY : (base + log2f(l)) * 0.693147180559945309f;
     }
@@ -262,8 +235,6 @@ __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const 
       uint2 raw[kSteps];
 #pragma unroll
       for (int e = 0; e < kSteps; ++e) raw[e] = lds64(from + st * S::staging + e * kStep * D);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar.taken[is_v][st]);
       if (turn > 0 && !warp_wait(&empty[at], (turn - 1) & 1, err, kErrTimeoutEmpty)) break;
       if (S::q_smem == 0 && is_v && i == 1 && !warp_wait(&bar.q_full, 0, err, kErrTimeoutEmpty)) break;  // Q has passed
 #pragma unroll
@@ -277,7 +248,12 @@ __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const 
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&full[at]);
+      if (lane == 0) {
+        mbar_arrive(&full[at]);
+        // only now: an arrival does not wait for loads before it whose values nothing has used, and the next copy would
+        // overtake them
+        mbar_arrive(&bar.taken[is_v][st]);
+      }
       if (++at == ring) at = 0, ++turn;
     }
   } else {

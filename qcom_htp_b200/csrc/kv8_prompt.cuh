@@ -80,6 +80,11 @@ __device__ __forceinline__ void pin(uint32_t (&x)[N]) {
 __device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+  uint4 r;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at) : "memory");
+  return r;
+}
 __device__ __forceinline__ uint2 lds64(uint32_t at) {
   uint2 r;
   asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(at) : "memory");
@@ -159,6 +164,18 @@ __device__ __forceinline__ void load_q(const Kv8Attn& a, int b, int h, long long
       head += kRows;
       while (head >= a.group) head -= a.group, ++t;
     }
+    uint32_t top[kBatch];
+    if (a.bf16) {
+      // bf16 magnitudes are ordered like their bits: the largest of the lane's, then of the row's.  A step of all rows at
+      // a time: shuffles keep their order, and a row after the other would wait for each.
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        top[i] = __vmaxu2(__vmaxu2(w[i].x & 0x7fff7fffu, w[i].y & 0x7fff7fffu), __vmaxu2(w[i].z & 0x7fff7fffu, w[i].w & 0x7fff7fffu));
+#pragma unroll
+      for (int o = 1; o < kLanes; o <<= 1)
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) top[i] = __vmaxu2(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+    }
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       const int r = warp * WARP_ROWS + (base + i) * kRows + sub;
@@ -166,19 +183,78 @@ __device__ __forceinline__ void load_q(const Kv8Attn& a, int b, int h, long long
       if (a.bf16) {
         float x[8];
         Vec<__nv_bfloat16>::load(w[i], x);
-        // bf16 magnitudes are ordered like their bits: the largest of the lane's, then of the row's
-        uint32_t top = __vmaxu2(__vmaxu2(w[i].x & 0x7fff7fffu, w[i].y & 0x7fff7fffu),
-                                __vmaxu2(w[i].z & 0x7fff7fffu, w[i].w & 0x7fff7fffu));
-#pragma unroll
-        for (int o = 1; o < kLanes; o <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
-        top = max(top & 0xffffu, top >> 16);
         float up;
-        row_factor(__uint_as_float(top << 16), up, down);
+        row_factor(__uint_as_float(max(top[i] & 0xffffu, top[i] >> 16) << 16), up, down);
         w[i] = make_uint4(pack_half2(x[0] * up, x[1] * up), pack_half2(x[2] * up, x[3] * up),
                           pack_half2(x[4] * up, x[5] * up), pack_half2(x[6] * up, x[7] * up));
       }
       *reinterpret_cast<uint4*>(img + (c >> 3) * kQPanel + swizzled(r, c & 7)) = w[i];
       if (c == 0) down_at[r] = down;
+    }
+  }
+}
+
+// A warp's 32 finished rows on their way out, 128 bytes of each at a time: a lane has a row in tensor memory, and stores of
+// one row's 16 bytes each would take 32 lines at a time.  They go through 4 KB of shared memory instead, and leave as whole
+// 128-byte pieces, four rows a store.
+struct RowsOut {
+  uint32_t stage;      // the warp's 4 KB
+  uint8_t* to[8];      // this lane's 16 bytes of rows lane / 8, lane / 8 + 4, ...; null: not there
+  // four 16-byte chunks of the lane's row, from chunk c0
+  __device__ __forceinline__ void fill(int lane, int c0, const uint32_t* x) const {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) sts128(stage + swizzled(lane, c0 + c), x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
+  }
+  __device__ __forceinline__ void flush(int lane, int byte) const {
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint4 v = lds128(stage + swizzled(4 * k + (lane >> 3), lane & 7));
+      if (to[k] != nullptr) *reinterpret_cast<uint4*>(to[k] + byte) = v;
+    }
+    __syncwarp();
+  }
+};
+
+// COLS columns (a multiple of 64) of the warp's rows (from column col0; O at o_at, or zeros), normalised to out or as they are to the parts.
+// rw: the warp's first row of the group; part0: its part.
+template <int D, int COLS>
+__device__ __forceinline__ void rows_out(const Kv8Attn& a, int b, int h, long long row0, int rw, int r1, long long part0, bool zero,
+                                         uint32_t o_at, int col0, float inv, uint32_t stage, int lane) {
+  RowsOut o;
+  o.stage = stage;
+  const bool whole = a.chunks == 1;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int i = 4 * k + (lane >> 3), r = rw + i, t = r / a.group, head = h * a.group + r - t * a.group;
+    uint8_t* p = whole ? reinterpret_cast<uint8_t*>(static_cast<uint16_t*>(a.out.data) + b * a.out.batch_stride +
+                                                    (row0 + t) * a.out.token_stride + head * a.out.head_stride + col0)
+                       : reinterpret_cast<uint8_t*>(a.part + (part0 + i) * D + col0);
+    o.to[k] = r < r1 ? p + (lane & 7) * 16 : nullptr;
+  }
+#pragma unroll 1
+  for (int c = 0; c < COLS; c += 32) {
+    uint32_t x[32];
+    if (zero) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) x[e] = 0;
+    } else {
+      tmem_ld32(o_at + c, x);
+      tmem_ld_wait();
+      pin(x);
+    }
+    if (whole) {
+#pragma unroll
+      for (int e = 0; e < 32; e += 2) {
+        const float u = __uint_as_float(x[e]) * inv, v = __uint_as_float(x[e + 1]) * inv;
+        x[e / 2] = a.bf16 ? Vec<__nv_bfloat16>::pack(u, v) : pack_half2(u, v);
+      }
+      o.fill(lane, (c & 32) / 8, x);
+      if (c & 32) o.flush(lane, 2 * (c - 32));
+    } else {
+      o.fill(lane, 0, x);
+      o.fill(lane, 4, x + 16);
+      o.flush(lane, 4 * c);
     }
   }
 }

@@ -196,43 +196,20 @@ __global__ void __launch_bounds__(Shape2<D>::threads, 1) kv8_prompt2_kernel(cons
       l = s_half[tiles & 1][slot][0][in_tile] + s_half[tiles & 1][slot][1][in_tile];
       const float base = m == -INFINITY ? 0.0f : m;
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const int rw = sr0 + wq * 32;
+      const long long part0 = part_row(a, b, h, rg, chunk) + slot * 128 + wq * 32, part = part0 + lane;
+      // K's images are free: every S has been computed.  Rows of
+      // head_dim 64 are one piece, which the first half's warp takes.
+      if (D == 128 || half == 0)
+        rows_out<D, 64>(a, b, h, row0, rw, sr1, part0, tiles == 0, o_at, half * 64, inv,
+                        smem_u32(k_img) + (D == 128 ? warp : slot * 4 + wq) * 4096, lane);
       const bool live = r < sr1;
-      const int t = r / a.group, head = h * a.group + r - t * a.group;
-      const long long part = part_row(a, b, h, rg, chunk) + slot * 128 + in_tile;
-      uint16_t* out = static_cast<uint16_t*>(a.out.data) + b * a.out.batch_stride + (row0 + t) * a.out.token_stride +
-                      head * a.out.head_stride + half * (D / 2);
-#pragma unroll 1
-      for (int c = 0; c < D / 64; ++c) {
-        uint32_t x[32];
-        if (tiles > 0) {
-          tmem_ld32(o_at + 32 * c, x);
-          tmem_ld_wait();
-          pin(x);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] = 0;
-        }
-        __syncwarp();
-        if (live && a.chunks == 1) {
-#pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            float v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(x[e + i]) * inv;
-            *reinterpret_cast<uint4*>(out + 32 * c + e) = a.bf16 ? Vec<__nv_bfloat16>::store(v) : Vec<__half>::store(v);
-          }
-        } else if (live) {
-          uint4* to = reinterpret_cast<uint4*>(a.part + part * D + half * (D / 2) + 32 * c);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) to[e] = make_uint4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
-        }
-        __syncwarp();
-      }
       if (half == 0 && live) {
         if (a.chunks > 1) {
           float* ml = a.part + part_rows(a) * D + 2 * part;
           ml[0] = base, ml[1] = l;
         } else if (a.lse != nullptr) {
+          const int t = r / a.group, head = h * a.group + r - t * a.group;
           const long long at = (a.seqs.start ? row0 : static_cast<long long>(b) * a.seqs.tokens) + t;
           a.lse[at * a.q_heads + head] = l == 0.0f ? -INFINITY : (base + log2f(l)) * 0.693147180559945309f;
         }
@@ -257,8 +234,6 @@ __global__ void __launch_bounds__(Shape2<D>::threads, 1) kv8_prompt2_kernel(cons
       uint2 raw[kSteps];
 #pragma unroll
       for (int e = 0; e < kSteps; ++e) raw[e] = lds64(from + at * S::staging + e * kStep * D);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar.taken[at]);
       if ((q & 1) == 0 && j >= 2)
         ok = warp_wait(q ? &bar.v_empty[st] : &bar.k_empty[st], ((j >> 1) - 1) & 1, err, kErrTimeoutEmpty);
       const uint32_t img = to + (q & 2 ? 2 * S::tile : 0) + st * S::tile + (q & 1) * (kUnit * 128);
@@ -271,6 +246,9 @@ __global__ void __launch_bounds__(Shape2<D>::threads, 1) kv8_prompt2_kernel(cons
       }
       fence_proxy_async_smem();
       __syncwarp();
+      // only now: an arrival does not wait for loads before it whose values nothing has used, and the next copy would
+      // overtake them
+      if (lane == 0) mbar_arrive(&bar.taken[at]);
       if ((q & 1) && lane == 0) mbar_arrive(q & 2 ? &bar.v_full[st] : &bar.k_full[st]);
     }
   } else {

@@ -352,7 +352,8 @@ def test_runs_repeat_bit_for_bit():
 
 
 @pytest.mark.parametrize("d", [64, 128, 256])
-@pytest.mark.parametrize("lengths,t,hq,bs", [([200, 333], 200, 4, 64), ([2000, 1333, 1000], 150, 16, 16), ([4000] * 9, 1, 8, 32)])
+@pytest.mark.parametrize("lengths,t,hq,bs", [([200, 333], 200, 4, 64), ([2000, 1333, 1000], 150, 16, 16), ([4000] * 9, 1, 8, 32),
+                                                ([4096], 4096, 32, 64)])
 def test_many_runs_give_the_same_bits(d, lengths, t, hq, bs):
     """The kernels' roles hand over through barriers: none may depend on who comes first."""
     blocks = sum(-(-n // bs) for n in lengths)
