@@ -9,6 +9,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "internal.h"
@@ -278,6 +279,17 @@ inline cudaError_t kv8_take_error(const void* symbol, int* code, cudaStream_t st
   if (e == cudaSuccess) e = cudaMemsetAsync(at, 0, sizeof(int), stream);
   if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
   return e;
+}
+// Runs `set` once per device (again where it failed).
+template <typename F>
+inline cudaError_t once_per_device(std::atomic<bool> (&done)[64], F set) {
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 0 && dev < 64 && done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+  const cudaError_t r = set();
+  if (r == cudaSuccess && dev >= 0 && dev < 64) done[dev].store(true, std::memory_order_release);
+  return r;
 }
 inline size_t kv8_part_bytes(const Kv8Attn& a) {
   if (a.chunks <= 1) return 0;

@@ -564,8 +564,10 @@ cudaError_t run(const Kv8Attn& a) {
   for (int i = 0; i < 2; ++i)
     if (!make_tmap_tiles_u8(&map[i], i ? a.pages.v : a.pages.k, D, 1ull << a.pages.bs_log2, tiles, D < 128 ? D : 128, 16, swizzle))
       return cudaErrorInvalidValue;
-  const cudaError_t e =
-      cudaFuncSetAttribute(kv8_decode_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Rg::smem);
+  static std::atomic<bool> done[64];
+  const cudaError_t e = once_per_device(done, [] {
+    return cudaFuncSetAttribute(kv8_decode_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Rg::smem);
+  });
   if (e != cudaSuccess) return e;
   const dim3 grid(static_cast<unsigned>(a.pages.heads) * a.row_groups, a.seqs.batch, a.chunks);
   kv8_decode_kernel<D, NT><<<grid, kWarps * 32, Rg::smem, a.stream>>>(a, map[0], map[1]);

@@ -371,7 +371,8 @@ cudaError_t prepare() {
 template <int D>
 cudaError_t run(const Kv8Attn& a) {
   using S = Shape<D>;
-  const cudaError_t e = prepare<D>();
+  static std::atomic<bool> done[64];
+  const cudaError_t e = once_per_device(done, prepare<D>);
   if (e != cudaSuccess) return e;
   const dim3 grid(static_cast<unsigned>(a.pages.heads) * a.chunks, a.seqs.batch, a.row_groups);
   kv8_prompt_kernel<D><<<grid, S::threads, S::smem, a.stream>>>(a);

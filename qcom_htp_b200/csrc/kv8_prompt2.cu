@@ -358,14 +358,22 @@ __global__ void __launch_bounds__(Shape2<D>::threads, 1) kv8_prompt2_kernel(cons
 }
 
 template <int D>
-cudaError_t run2(const Kv8Attn& a) {
+cudaError_t prepare2() {
   using S = Shape2<D>;
   cudaError_t e = cudaFuncSetAttribute(kv8_prompt2_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem);
   if (e != cudaSuccess) return e;
   cudaFuncAttributes at;
   if ((e = cudaFuncGetAttributes(&at, kv8_prompt2_kernel<D>)) != cudaSuccess) return e;
   // the roles' registers come out of what the launch has: more than that would be waited for without end
-  if (at.numRegs != S::regs) return cudaErrorInvalidConfiguration;
+  return at.numRegs == S::regs ? cudaSuccess : cudaErrorInvalidConfiguration;
+}
+
+template <int D>
+cudaError_t run2(const Kv8Attn& a) {
+  using S = Shape2<D>;
+  static std::atomic<bool> done[64];
+  const cudaError_t e = once_per_device(done, prepare2<D>);
+  if (e != cudaSuccess) return e;
   const dim3 grid(static_cast<unsigned>(a.pages.heads) * a.chunks, a.seqs.batch, a.row_groups);
   kv8_prompt2_kernel<D><<<grid, S::threads, S::smem, a.stream>>>(a);
   return cudaGetLastError();

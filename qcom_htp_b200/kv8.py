@@ -32,6 +32,7 @@ _DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 # QhtpKv8Move and QhtpKv8Attention, packed in one call (native sizes and alignment)
 _MOVE = struct.Struct("@4Pq4I 2P2q4I P P3q P3q 2I P")
 _ATTENTION = struct.Struct("@4Pq4I 2P2q4I P P3q P3q P 4I f I P N P")
+_TAIL = struct.Struct("@P N P")  # workspace, its size, stream
 
 
 class Kv8Cache(NamedTuple):
@@ -54,33 +55,36 @@ class Kv8Cache(NamedTuple):
 
 
 def _cache_fields(cache):
+    """The cache's fields of the packed structures, and its device."""
     k, v, ks, vs = cache
     shape = k.shape
-    if not (k.is_cuda and len(shape) == 4 and v.shape == shape and ks.shape == shape[:2] and vs.shape == shape[:2]):
-        raise ValueError("the cache is int8 [num_blocks, kv_heads, block_size, head_dim] twice, float32 [num_blocks, kv_heads] "
-                         "twice, on a CUDA device")
+    if len(shape) != 4 or v.shape != shape or ks.shape != shape[:2] or vs.shape != ks.shape:
+        raise ValueError("the cache is int8 [num_blocks, kv_heads, block_size, head_dim] twice and float32 [num_blocks, kv_heads] twice")
     if not (k.dtype is v.dtype is torch.int8 and ks.dtype is vs.dtype is torch.float32):
         raise TypeError("the cache's codes must be int8 and its scales float32")
-    dev = k.device
     if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
         raise ValueError("the cache's tensors must be contiguous")
-    if v.device != dev or ks.device != dev or vs.device != dev:
-        raise ValueError("the cache's tensors must be on one device")
+    dev = k.device
+    if not k.is_cuda or v.device != dev or ks.device != dev or vs.device != dev:
+        raise ValueError("the cache's tensors must be on one CUDA device")
     return (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), shape[0], shape[1], shape[3], shape[2], 0), dev
 
 
 def _ints(name, t, n, dev):
-    if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or t.device != dev:
+    if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous() or t.device != dev:
         raise ValueError(f"{name} must be a contiguous int32 tensor of {n} elements on the cache's device")
     return t.data_ptr()
 
 
 def _seqs_fields(table, seq_start, tokens, total, dev):
-    if table.dtype is not torch.int32 or table.dim() != 2 or table.device != dev or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise ValueError("block_table must be an int32 [batch, blocks] tensor on the cache's device, its rows contiguous")
-    b, width = table.shape
-    start = 0 if seq_start is None else _ints("seq_start", seq_start, b + 1, dev)
-    return table.data_ptr(), start, table.stride(0), total, width, b, tokens, 0
+    shape = table.shape
+    if table.dtype is not torch.int32 or len(shape) != 2 or table.device != dev:
+        raise ValueError("block_table must be an int32 [batch, blocks] tensor on the cache's device")
+    b, width = shape
+    row, col = table.stride()
+    if col != 1 and width > 1:
+        raise ValueError("block_table's rows must be contiguous")
+    return table.data_ptr(), 0 if seq_start is None else _ints("seq_start", seq_start, b + 1, dev), row, total, width, b, tokens, 0
 
 
 def _rows_fields(name, t, heads, head_dim, dtype, dev, ragged):
@@ -97,8 +101,8 @@ def _rows_fields(name, t, heads, head_dim, dtype, dev, ragged):
     if ragged:
         bs, ts, hs = 0, s[0], s[1]
     else:
-        bs, ts, hs = s[0], s[1], s[2]
-    if (ptr | (bs | ts | hs) * t.element_size()) & 15:
+        bs, ts, hs, _ = s
+    if (ptr | (bs | ts | hs) * (4 if dtype is torch.float32 else 2)) & 15:
         raise ValueError(f"{name}: every head must start on a multiple of 16 bytes")
     return ptr, bs, ts, hs
 
@@ -110,11 +114,14 @@ def _counts(t, seq_start, most, what):
             raise ValueError(f"{what} must be [batch, tokens, heads, head_dim], or come with seq_start")
         return t.shape[1], 0
     total = t.shape[0]
-    return total if most is None else min(int(most), total), total
+    return total if most is None else max(0, min(int(most), total)), total
 
 
 # the current stream's handle without making a Stream object (a tenth of the time), where torch has it
 _current = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _on(stream, dev):
@@ -126,22 +133,30 @@ def _on(stream, dev):
     return stream.cuda_stream
 
 
-def _call(fn, name, dev, *args):
-    if dev.index != torch.cuda.current_device():
+def _call(fn, name, dev, arg):
+    if dev.index != _device():
         with torch.cuda.device(dev):
-            st = fn(*args)
+            st = fn(arg)
     else:
-        st = fn(*args)
+        st = fn(arg)
     if st:
         L.check(name, st)
 
 
-def _empty(like, shape, dtype, dev, stream):
-    """A tensor of the allocator's beside `like`, to be used on `stream`."""
+def _empty(like, shape, dtype, stream):
+    """A tensor of the allocator's on the device of `like`, to be used on `stream`."""
     if stream is None:
         return like.new_empty(shape, dtype=dtype)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=dev)
+        return like.new_empty(shape, dtype=dtype)
+
+
+def _like(t, stream):
+    """_empty of a contiguous tensor's own shape and type, in half the time."""
+    if stream is None:
+        return torch.empty_like(t)
+    with torch.cuda.stream(stream):
+        return torch.empty_like(t)
 
 
 def kv8_write(cache, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, past: torch.Tensor, *,
@@ -193,7 +208,8 @@ def kv8_read(cache, block_table: torch.Tensor, first: torch.Tensor, tokens: int 
         shape, total = (block_table.shape[0], tokens, heads, d), 0
     sf = _seqs_fields(block_table, seq_start, tokens, total, dev)
     pf = _ints("first", first, sf[5], dev)
-    k, v = _empty(first, shape, dtype, dev, stream), _empty(first, shape, dtype, dev, stream)
+    k = _empty(first, shape, dtype, stream)
+    v = _like(k, stream)
     ts = heads * d
     arg = _MOVE.pack(*cf, *sf, pf, k.data_ptr(), 0 if ragged else tokens * ts, ts, d,
                      v.data_ptr(), 0 if ragged else tokens * ts, ts, d, _DTYPE[dtype], 0, _on(stream, dev))
@@ -235,21 +251,23 @@ def kv8_attention(q: torch.Tensor, cache, block_table: torch.Tensor, lengths: to
         scale = d ** -0.5
     if not 0.0 < scale < float("inf"):
         raise ValueError("scale must be finite and above 0")
-    if out is None:
-        out = _empty(q, shape, dtype, dev, stream)
+    if out is None:  # contiguous
+        out, ts = _like(q, stream) if q.is_contiguous() else _empty(q, shape, dtype, stream), heads * d
+        ro = out.data_ptr(), 0 if ragged else tokens * ts, ts, d
     elif out.shape != shape:
         raise ValueError("out must have q's shape")
-    ro = _rows_fields("out", out, heads, d, dtype, dev, ragged)
-    lse = _empty(q, shape[:-1], torch.float32, dev, stream) if return_lse else None
+    else:
+        ro = _rows_fields("out", out, heads, d, dtype, dev, ragged)
+    lse = _empty(q, shape[:-1], torch.float32, stream) if return_lse else None
     reach = sf[4] * cf[7]
-    reach = reach if max_len is None else max(0, min(int(max_len), reach))
+    if max_len is not None:
+        reach = max(0, min(int(max_len), reach))
     handle = _on(stream, dev)
-    fields = (*cf, *sf, lf, *rq, *ro, lse.data_ptr() if return_lse else 0, _DTYPE[dtype], heads, 1 if causal else 0, window,
-              scale, reach)
-    arg = _ATTENTION.pack(*fields, 0, 0, handle)
+    arg = _ATTENTION.pack(*cf, *sf, lf, *rq, *ro, lse.data_ptr() if return_lse else 0, _DTYPE[dtype], heads, 1 if causal else 0,
+                          window, scale, reach, 0, 0, handle)
     need = L.lib.qhtp_kv8_attention_workspace_bytes(arg)
     if need:
-        ws = _empty(q, need, torch.uint8, dev, stream)
-        arg = _ATTENTION.pack(*fields, ws.data_ptr(), need, handle)
+        ws = _empty(q, (need,), torch.uint8, stream)
+        arg = arg[:-_TAIL.size] + _TAIL.pack(ws.data_ptr(), need, handle)
     _call(L.lib.qhtp_kv8_attention, "qhtp_kv8_attention", dev, arg)
     return (out, lse) if return_lse else out
