@@ -10,7 +10,7 @@
 //   K and V converters (a warpgroup each) write them as f16 into 128-byte-swizzled images [key][64 head_dim], two to
 //     four units ahead: K-major for Q K^T, and the same bytes MN-major for P V;
 //   one warp issues the MMAs: S = Q K^T into tensor memory, O += P V with P read from tensor memory;
-//   a softmax warpgroup, a thread per row: S from tensor memory, P back over it as f16.
+//   two softmax warpgroups, two threads per row with 32 keys each: S from tensor memory, P back over it as f16.
 // There are two S buffers, so that the softmax of one unit runs under the MMAs of its neighbours.  Q stands in tensor
 // memory: an MMA of 64 columns then reads 2 KB of shared memory where it would read 6.
 //
@@ -37,13 +37,12 @@ struct Shape {
   static constexpr int q_tile = panels * kQPanel;
   // Q's image on its way to tensor memory: where there is no room for it, it passes through V's last units
   static constexpr int q_smem = D == 256 ? 0 : q_tile;
-  static constexpr int smem = q_smem + (k_units + v_units) * unit + 2 * depth * staging + 1024;
-  static_assert(smem + 2048 <= 227 * 1024, "shared memory");
+  static constexpr int data = q_smem + (k_units + v_units) * unit + 2 * depth * staging;
   static_assert(q_smem != 0 || q_tile <= (v_units - 1) * unit, "Q in V's units");
-  static constexpr int threads = 512;
+  static constexpr int threads = 640;
   // registers of a thread: at launch (the most that the threads leave room for), and by role
-  static constexpr int regs = 128, softmax_regs = 176, convert_regs = 112, issue_regs = 96;
-  static_assert(softmax_regs + 2 * convert_regs + issue_regs <= 4 * regs, "registers");
+  static constexpr int regs = 96, softmax_regs = 112, convert_regs = 96, issue_regs = 64;
+  static_assert(2 * softmax_regs + 2 * convert_regs + issue_regs <= 5 * regs, "registers");
   // tensor memory columns: two S buffers of 64 from 0, Q, O
   static constexpr int q_col = 128, o_col = 256;
   static_assert(q_col + D / 2 <= o_col && o_col + D <= 512, "tensor memory");
@@ -53,17 +52,28 @@ struct Barriers {
   uint64_t q_full, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_full[2], pv_done, drained, staged[2][4], taken[2][4];
 };
 
+struct Small {
+  float4 scale[8][4];     // (c, log2 w, 1 / w, care) of a unit's 16-key groups, eight units deep
+  // [turn][half][row]: a half row's maximum, at the end its sum; at the start, before half[1] is in use, half[1][0] has
+  // the rows' factors
+  float half[2][2][128];
+  Barriers bar;
+  uint32_t tmem;
+};
+
 __device__ int g_error;  // a wait that gave up leaves its code here
 
 template <int D>
 __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const Kv8Attn a) {
   using S = Shape<D>;
   int* const err = &g_error;
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ Barriers bar;
-  __shared__ uint32_t s_tmem;
-  __shared__ float s_down[128];
-  __shared__ float4 s_scale[8][4];       // (c, log2 w, 1 / w, care) of a unit's 16-key groups, eight units deep
+  extern __shared__ __align__(1024) uint8_t smem[];
+  static_assert(S::data + sizeof(Small) <= 227 * 1024, "shared memory");
+  Small& small = *reinterpret_cast<Small*>(smem + S::data);
+  Barriers& bar = small.bar;
+  float(&s_half)[2][2][128] = small.half;
+  float(&s_down)[128] = small.half[1][0];
+  float4(&s_scale)[8][4] = small.scale;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // heads fastest, the longest row groups (the last of a causal sequence) first
@@ -80,15 +90,14 @@ __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const 
   const int units = keys.lo < keys.hi ? (keys.hi - keys.lo + kKeys - 1) / kKeys : 0;
   if (units == 0 && chunk > 0) return;
 
-  uint8_t* const smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint8_t* const k_img = smem + S::q_smem;
   uint8_t* const v_img = k_img + S::k_units * S::unit;
   uint8_t* const stage_img = v_img + S::v_units * S::unit;
   uint8_t* const q_img = S::q_smem ? smem : v_img + S::unit;
 
-  constexpr int kConvK = 4, kConvV = 8, kMma = 12, kCopyK = 13, kCopyV = 14, kScale = 15;  // first warps of the roles
+  constexpr int kConvK = 8, kConvV = 12, kMma = 16, kCopyK = 17, kCopyV = 18, kScale = 19;  // first warps of the roles
   if (warp == kMma) {
-    tmem_alloc(&s_tmem, 512);
+    tmem_alloc(&small.tmem, 512);
     if (lane == 0) {
       for (int i = 0; i < 4; ++i) {
         mbar_init(&bar.k_full[i], 5);  // the converter warps, and the one that brings the scales
@@ -99,9 +108,9 @@ __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const 
       }
       for (int i = 0; i < 2; ++i) {
         mbar_init(&bar.s_full[i], 2);  // the MMAs, and the issuing thread's own arrival
-        mbar_init(&bar.p_full[i], 128);
+        mbar_init(&bar.p_full[i], 256);
       }
-      mbar_init(&bar.q_full, 128);
+      mbar_init(&bar.q_full, 256);
       mbar_init(&bar.pv_done, 1);
       mbar_init(&bar.drained, 1);
       fence_barrier_init();
@@ -111,21 +120,21 @@ __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = s_tmem;
+  const uint32_t tmem = small.tmem;
 
   if (warp < kConvK) {
-    // ------------------------------------------------------------------------------- softmax, a thread per row
+    // ------------------------------------------------------------------------------- softmax, two threads per row
     reg_alloc<S::softmax_regs>();
-    const int in_tile = warp * 32 + lane, r = r0 + in_tile;
-    const uint32_t lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
-    const uint32_t o_at = lanes + S::o_col;
+    const int half = warp >> 2, wq = warp & 3, in_tile = wq * 32 + lane, r = r0 + in_tile;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(wq * 32) << 16);
+    const uint32_t o_at = lanes + S::o_col + half * (D / 2);
     float m = -INFINITY, l = 0.0f;
     if (units > 0) {
-      load_q<D>(a, b, h, row0, r0, r1, q_img, s_down, warp, lane);
-      __syncwarp();
+      load_q<D, 16>(a, b, h, row0, r0, r1, q_img, s_down, warp, lane);
+      named_barrier(1, 256);
       const float down = s_down[in_tile];
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
+      for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {
         uint32_t x[16];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -143,32 +152,32 @@ __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const 
       // every row sees the keys [all_lo, all_hi)
       const int all_hi = a.causal ? min(keys.hi, len - T + r0 / a.group + 1) : keys.hi;
       const int all_lo = a.window ? len - T + (r1 - 1) / a.group - a.window + 1 : 0;
+      bool ok = true;
       for (int i = 0; i < units; ++i) {
         const int buf = i & 1;
-        const uint32_t s_at = lanes + buf * 64;
-        if (!warp_wait(&bar.s_full[buf], (i >> 1) & 1, err, kErrTimeoutAccum)) break;
+        const uint32_t s_at = lanes + buf * 64 + half * 32;
+        // after a wait that gave up the rows are lost, but every warp still passes every named barrier
+        ok = ok && warp_wait(&bar.s_full[buf], (i >> 1) & 1, err, kErrTimeoutAccum);
         tc_fence_after();
-        uint32_t x[2][32];
-        tmem_ld32(s_at, x[0]);
-        tmem_ld32(s_at + 32, x[1]);
-        const int key0 = keys.lo + i * kKeys;
-        const View k{s_scale[i & 7], down, row_lo - key0, row_hi - key0};
-        const bool careful = key0 + kKeys > all_hi || key0 < all_lo || k.scale[0].w != 0.0f;
+        uint32_t x[32], w[16];
+        tmem_ld32(s_at, x);
+        const int key0 = keys.lo + i * kKeys, col0 = key0 + half * 32;
+        const View k{&s_scale[i & 7][2 * half], down, row_lo - col0, row_hi - col0};
+        const bool careful = key0 + kKeys > all_hi || key0 < all_lo || s_scale[i & 7][0].w != 0.0f;
         tmem_ld_wait();
-        pin(x[0]), pin(x[1]);
-        float top = m;
-        if (careful)
-          top = row_max<true>(k, 0, x[0], top), top = row_max<true>(k, 32, x[1], top);
-        else
-          top = row_max<false>(k, 0, x[0], top), top = row_max<false>(k, 32, x[1], top);
-        // raise m where it pays; rows of a warp move together
+        pin(x);
+        float top = careful ? row_max<true>(k, 0, x, m) : row_max<false>(k, 0, x, m);
+        s_half[buf][half][in_tile] = top;
+        named_barrier(1, 256);
+        top = fmaxf(top, s_half[buf][half ^ 1][in_tile]);
+        // raise m where it pays; rows of a warp move together, and its two halves alike
         if (__any_sync(0xffffffffu, top > m + kGrow || (m == -INFINITY && top != -INFINITY))) {
           const float alpha = m == -INFINITY ? 0.0f : ex2(m - top);
           if (i > 0) {
-            if (!warp_wait(&bar.pv_done, (i - 1) & 1, err, kErrTimeoutAccum)) break;
+            ok = ok && warp_wait(&bar.pv_done, (i - 1) & 1, err, kErrTimeoutAccum);
             tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < D / 16; ++c) {
+            for (int c = 0; c < D / 32; ++c) {
               uint32_t o[16];
               tmem_ld16(o_at + 16 * c, o);
               tmem_ld_wait();
@@ -182,30 +191,30 @@ __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const 
           m = top;
         }
         const float base = m == -INFINITY ? 0.0f : m;
-        uint32_t w[2][16];
-        if (careful)
-          l = row_exp<true>(k, 0, x[0], base, l, w[0]), l = row_exp<true>(k, 32, x[1], base, l, w[1]);
-        else
-          l = row_exp<false>(k, 0, x[0], base, l, w[0]), l = row_exp<false>(k, 32, x[1], base, l, w[1]);
-        tmem_st16(s_at, w[0]);
-        tmem_st16(s_at + 16, w[1]);
+        l = careful ? row_exp<true>(k, 0, x, base, l, w) : row_exp<false>(k, 0, x, base, l, w);
+        tmem_st16(s_at, w);
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&bar.p_full[buf]);
       }
       // the last product may be two phases ahead of what this warp has seen (S of a unit comes before P V of the one before
       // it), and a parity tells only one: both are waited for
-      if (units > 1) warp_wait(&bar.pv_done, (units - 2) & 1, err, kErrTimeoutAccum);
-      warp_wait(&bar.pv_done, (units - 1) & 1, err, kErrTimeoutAccum);
+      if (ok && units > 1) ok = warp_wait(&bar.pv_done, (units - 2) & 1, err, kErrTimeoutAccum);
+      if (ok) warp_wait(&bar.pv_done, (units - 1) & 1, err, kErrTimeoutAccum);
       tc_fence_after();
     }
-    // the rows
+    // the row's sum, and each half's columns of it
+    s_half[units & 1][half][in_tile] = l;
+    named_barrier(1, 256);
+    l = s_half[units & 1][0][in_tile] + s_half[units & 1][1][in_tile];
     const float base = m == -INFINITY ? 0.0f : m;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const long long part0 = part_row(a, b, h, rg, chunk) + warp * 32, part = part0 + lane;
-    // K's images are free: every S has been computed
-    rows_out<D, D>(a, b, h, row0, r0 + warp * 32, r1, part0, units == 0, o_at, 0, inv, smem_u32(k_img) + warp * 4096, lane);
-    const bool live = r < r1;
+    const long long part0 = part_row(a, b, h, rg, chunk) + wq * 32, part = part0 + lane;
+    // K's images are free: every S has been computed.  Rows of head_dim 64 are one piece, which the first half's warp takes.
+    if (D > 64 || half == 0)
+      rows_out<D, (D > 64 ? D / 2 : 64)>(a, b, h, row0, r0 + wq * 32, r1, part0, units == 0, o_at, D > 64 ? half * (D / 2) : 0, inv,
+                                         smem_u32(k_img) + warp * 4096, lane);
+    const bool live = r < r1 && half == 0;
     if (live && a.chunks > 1) {
       float* ml = a.part + part_rows(a) * D + 2 * part;
       ml[0] = base, ml[1] = l;
@@ -339,7 +348,7 @@ __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const 
           const uint32_t vd = v_desc + at * (S::unit >> 4);
 #pragma unroll
           for (int e = 0; e < kKeys / 16; ++e)
-            mma_ts(leader, tm + S::o_col, tm + buf * 64 + 8 * e, vd + e * (2048 >> 4), id_pv, i > 1 || e != 0);
+            mma_ts(leader, tm + S::o_col, tm + buf * 64 + (e >> 1) * 32 + (e & 1) * 8, vd + e * (2048 >> 4), id_pv, i > 1 || e != 0);
           commit(leader, smem_u32(&bar.pv_done));
           commit(leader, smem_u32(&bar.v_empty[at]));
         }
@@ -359,7 +368,7 @@ __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const 
 template <int D>
 cudaError_t prepare() {
   using S = Shape<D>;
-  cudaError_t e = cudaFuncSetAttribute(kv8_prompt_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem);
+  cudaError_t e = cudaFuncSetAttribute(kv8_prompt_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (S::data + static_cast<int>(sizeof(Small))));
   if (e != cudaSuccess) return e;
   cudaFuncAttributes at;
   if ((e = cudaFuncGetAttributes(&at, kv8_prompt_kernel<D>)) != cudaSuccess) return e;
@@ -375,7 +384,7 @@ cudaError_t run(const Kv8Attn& a) {
   const cudaError_t e = once_per_device(done, prepare<D>);
   if (e != cudaSuccess) return e;
   const dim3 grid(static_cast<unsigned>(a.pages.heads) * a.chunks, a.seqs.batch, a.row_groups);
-  kv8_prompt_kernel<D><<<grid, S::threads, S::smem, a.stream>>>(a);
+  kv8_prompt_kernel<D><<<grid, S::threads, (S::data + static_cast<int>(sizeof(Small))), a.stream>>>(a);
   return cudaGetLastError();
 }
 
