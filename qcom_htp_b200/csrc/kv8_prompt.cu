@@ -27,27 +27,6 @@ namespace {
 constexpr int kKeys = 64;              // keys of a unit
 constexpr int kPanel = kKeys * 128;    // bytes of a [64 keys][64 f16] swizzled image
 
-template <int D>
-struct Shape {
-  static constexpr int panels = D / 64;
-  static constexpr int unit = panels * kPanel;                  // 64 keys of K or V
-  static constexpr int k_units = D == 256 ? 2 : 4, v_units = D == 256 ? 3 : 4;
-  static constexpr int depth = D == 256 ? 2 : 4;                // staging buffers of K, and of V
-  static constexpr int staging = kKeys * D;                     // one of them
-  static constexpr int q_tile = panels * kQPanel;
-  // Q's image on its way to tensor memory: where there is no room for it, it passes through V's last units
-  static constexpr int q_smem = D == 256 ? 0 : q_tile;
-  static constexpr int data = q_smem + (k_units + v_units) * unit + 2 * depth * staging;
-  static_assert(q_smem != 0 || q_tile <= (v_units - 1) * unit, "Q in V's units");
-  static constexpr int threads = 640;
-  // registers of a thread: at launch (the most that the threads leave room for), and by role
-  static constexpr int regs = 96, softmax_regs = 112, convert_regs = 96, issue_regs = 64;
-  static_assert(2 * softmax_regs + 2 * convert_regs + issue_regs <= 5 * regs, "registers");
-  // tensor memory columns: two S buffers of 64 from 0, Q, O
-  static constexpr int q_col = 128, o_col = 256;
-  static_assert(q_col + D / 2 <= o_col && o_col + D <= 512, "tensor memory");
-};
-
 struct Barriers {
   uint64_t q_full, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_full[2], pv_done, drained, staged[2][4], taken[2][4];
 };
@@ -61,6 +40,29 @@ struct Small {
   uint32_t tmem;
 };
 
+template <int D>
+struct Shape {
+  static constexpr int panels = D / 64;
+  static constexpr int unit = panels * kPanel;                  // 64 keys of K or V
+  static constexpr int k_units = D == 256 ? 2 : 4, v_units = D == 256 ? 3 : 4;
+  static constexpr int depth = D == 256 ? 2 : 4;                // staging buffers of K, and of V
+  static constexpr int staging = kKeys * D;                     // one of them
+  static constexpr int q_tile = panels * kQPanel;
+  // Q's image on its way to tensor memory: where there is no room for it, it passes through V's last units
+  static constexpr int q_smem = D == 256 ? 0 : q_tile;
+  static constexpr int data = q_smem + (k_units + v_units) * unit + 2 * depth * staging;
+  static constexpr int smem = data + sizeof(Small);
+  static_assert(smem <= 227 * 1024, "shared memory");
+  static_assert(q_smem != 0 || q_tile <= (v_units - 1) * unit, "Q in V's units");
+  static constexpr int threads = 640;
+  // registers of a thread: at launch (the most that the threads leave room for), and by role
+  static constexpr int regs = 96, softmax_regs = 112, convert_regs = 96, issue_regs = 64;
+  static_assert(2 * softmax_regs + 2 * convert_regs + issue_regs <= 5 * regs, "registers");
+  // tensor memory columns: two S buffers of 64 from 0, Q, O
+  static constexpr int q_col = 128, o_col = 256;
+  static_assert(q_col + D / 2 <= o_col && o_col + D <= 512, "tensor memory");
+};
+
 __device__ int g_error;  // a wait that gave up leaves its code here
 
 template <int D>
@@ -68,7 +70,6 @@ __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const 
   using S = Shape<D>;
   int* const err = &g_error;
   extern __shared__ __align__(1024) uint8_t smem[];
-  static_assert(S::data + sizeof(Small) <= 227 * 1024, "shared memory");
   Small& small = *reinterpret_cast<Small*>(smem + S::data);
   Barriers& bar = small.bar;
   float(&s_half)[2][2][128] = small.half;
@@ -368,7 +369,7 @@ __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const 
 template <int D>
 cudaError_t prepare() {
   using S = Shape<D>;
-  cudaError_t e = cudaFuncSetAttribute(kv8_prompt_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (S::data + static_cast<int>(sizeof(Small))));
+  cudaError_t e = cudaFuncSetAttribute(kv8_prompt_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem);
   if (e != cudaSuccess) return e;
   cudaFuncAttributes at;
   if ((e = cudaFuncGetAttributes(&at, kv8_prompt_kernel<D>)) != cudaSuccess) return e;
@@ -384,7 +385,7 @@ cudaError_t run(const Kv8Attn& a) {
   const cudaError_t e = once_per_device(done, prepare<D>);
   if (e != cudaSuccess) return e;
   const dim3 grid(static_cast<unsigned>(a.pages.heads) * a.chunks, a.seqs.batch, a.row_groups);
-  kv8_prompt_kernel<D><<<grid, S::threads, (S::data + static_cast<int>(sizeof(Small))), a.stream>>>(a);
+  kv8_prompt_kernel<D><<<grid, S::threads, S::smem, a.stream>>>(a);
   return cudaGetLastError();
 }
 

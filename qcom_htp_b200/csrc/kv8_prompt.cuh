@@ -8,8 +8,6 @@ namespace {
 
 constexpr int kQPanel = 128 * 128;     // bytes of a [128 rows][64 f16] image of Q
 constexpr float kGrow = 8.0f;          // log2 of how far p may pass 1 before m follows
-// pairs of a 16-key group whose exponentials are computed by polynomial, a bit each
-constexpr uint32_t kPoly = 0x00;
 
 template <int N>
 __device__ __forceinline__ void reg_alloc() {
@@ -25,7 +23,7 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 __device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
-// (a.x * b + c, a.y * b + c) in one instruction
+// (x * b + c, y * b + c) in one instruction
 __device__ __forceinline__ float2 fma2(float x, float y, float b, float c) {
   float2 r;
   asm("{\n\t.reg .b64 u, v, w, z;\n\t"
@@ -45,31 +43,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "=f"(r.x), "=f"(r.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float c) {
-  float2 r;
-  asm("{\n\t.reg .b64 u, v, w, z;\n\t"
-      "mov.b64 u, {%2, %3};\n\tmov.b64 v, {%4, %5};\n\tmov.b64 w, {%6, %6};\n\t"
-      "fma.rn.f32x2 z, u, v, w;\n\t"
-      "mov.b64 {%0, %1}, z;\n\t}"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c));
-  return r;
-}
-// 2^t of a pair on the FMA pipe: t = n + f with n the nearest integer (it is left in the low bits of t + 1.5 2^23)
-// and |f| <= 1/2, 2^f by the degree-4 polynomial of least relative error there (2.6e-6, found by Remez exchange), n added
-// to the exponent.  t below -126 counts as -126.
-__device__ __forceinline__ float2 ex2_poly(float2 t) {
-  t.x = fmaxf(t.x, -126.0f), t.y = fmaxf(t.y, -126.0f);
-  const float2 big = add2(t, make_float2(12582912.0f, 12582912.0f));
-  const float2 n = add2(big, make_float2(-12582912.0f, -12582912.0f));
-  const float2 f = add2(t, make_float2(-n.x, -n.y));
-  float2 p = fma2(f.x, f.y, 0.009570102207362652f, 0.05591785907745361f);
-  p = fma2(p, f, 0.240247443318367f);
-  p = fma2(p, f, 0.6931217908859253f);
-  p = fma2(p, f, 0.9999992847442627f);
-  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(big.x) << 23)),
-                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(big.y) << 23)));
 }
 // Keeps uses of what tcgen05.ld wrote behind the wait for it: the wait itself does not name the registers.
 template <int N>
@@ -142,7 +115,7 @@ __device__ __forceinline__ uint32_t swizzled(int r, int c) {
 
 // The rows of one slot as f16 into its image, rows of bf16 scaled by a power of two each.  D / 8 lanes a row, all of a
 // warp's rows in flight at once.
-template <int D, int WARP_ROWS = 32>
+template <int D, int WARP_ROWS>
 __device__ __forceinline__ void load_q(const Kv8Attn& a, int b, int h, long long row0, int r0, int r1, uint8_t* img,
                                        float* down_at, int warp, int lane) {
   constexpr int kLanes = D / 8, kRows = 32 / kLanes;  // rows of a load
@@ -216,8 +189,8 @@ struct RowsOut {
   }
 };
 
-// COLS columns (a multiple of 64) of the warp's rows (from column col0; O at o_at, or zeros), normalised to out or as they are to the parts.
-// rw: the warp's first row of the group; part0: its part.
+// COLS columns (a multiple of 64) of the warp's rows, from column col0 (O at o_at, or zeros): normalised to out, or as they
+// are to the parts.  rw: the warp's first row of the group; part0: its part.
 template <int D, int COLS>
 __device__ __forceinline__ void rows_out(const Kv8Attn& a, int b, int h, long long row0, int rw, int r1, long long part0, bool zero,
                                          uint32_t o_at, int col0, float inv, uint32_t stage, int lane) {
@@ -309,10 +282,7 @@ __device__ __forceinline__ float row_exp(const View& k, int col0, const uint32_t
 #pragma unroll
     for (int e = 0; e < 16; e += 2) {
       float2 t = fma2(__uint_as_float(v[e]), __uint_as_float(v[e + 1]), f, off);
-      if (!CAREFUL && kPoly >> (e / 2) & 1)
-        t = ex2_poly(t);
-      else
-        t.x = ex2(t.x), t.y = ex2(t.y);
+      t.x = ex2(t.x), t.y = ex2(t.y);
       if constexpr (CAREFUL) {
         const int col = col0 + 16 * c + e;
         t.x = col < k.hi && col >= k.lo ? t.x : 0.0f;
