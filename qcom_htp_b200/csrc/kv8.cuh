@@ -161,9 +161,11 @@ struct Kv8Attn {
   float scale_log2;       // softmax scale * log2(e)
   int max_len;            // the caller's bound on the lengths (sizes the grid only)
   int prompt;             // kv8_prompt.cu, else kv8_decode.cu
-  // a launch's plan: rows per CTA, row groups of a sequence, keys per chunk, chunks
-  int tile_rows, row_groups, chunk, chunks;
-  float* part;            // workspace (chunks > 1): unnormalised rows, then their maxima and sums
+  // A launch's plan: rows per CTA, row groups of a sequence (the most of any), and how the keys are cut.  fit > 0: into
+  // chunks that the kernel sizes by the lengths, so that they are at most `fit` CTAs, of `chunk` keys at the least
+  // (fit_place); fit = 0: into `chunks` of `chunk` keys, on a grid sized by max_len.
+  int tile_rows, row_groups, chunk, chunks, fit;
+  float* part;            // workspace: unnormalised rows, then their maxima and sums, then (fit) the sequences' cuts
   cudaStream_t stream;
 };
 
@@ -184,18 +186,136 @@ __device__ __forceinline__ int seq_length(const Kv8Attn& a, int b) {
   const int len = max(a.lengths[b], 0);
   return len < cap ? len : static_cast<int>(cap);
 }
-// Chunk c of a span: chunks start at a multiple of 32 keys, and the last takes what is left.
-__device__ __forceinline__ Span chunk_span(const Kv8Attn& a, const Span& s, int c) {
-  const long long lo = (s.lo & ~31) + static_cast<long long>(c) * a.chunk;
-  const long long hi = c == a.chunks - 1 ? s.hi : min(static_cast<long long>(s.hi), lo + a.chunk);
+// What a CTA works on: chunk `chunk` of `chunks`, `keys` long, of a (sequence, kv head, row group); `part`: its first row
+// in the parts.
+struct Place {
+  int b, h, rg, chunk, chunks, keys;
+  long long part;
+};
+// Chunk of a span: chunks start at a multiple of 32 keys, and the last takes what is left.
+__device__ __forceinline__ Span chunk_span(const Place& p, const Span& s) {
+  const long long lo = (s.lo & ~31) + static_cast<long long>(p.chunk) * p.keys;
+  const long long hi = p.chunk == p.chunks - 1 ? s.hi : min(static_cast<long long>(s.hi), lo + p.keys);
   return lo < hi ? Span{static_cast<int>(lo), static_cast<int>(hi)} : Span{0, 0};
 }
 // Offset of a (sequence, kv head, row group, chunk) part in rows.
 __device__ __forceinline__ long long part_row(const Kv8Attn& a, int b, int h, int rg, int c) {
   return (((static_cast<long long>(b) * a.pages.heads + h) * a.row_groups + rg) * a.chunks + c) * a.tile_rows;
 }
-__device__ __forceinline__ long long part_rows(const Kv8Attn& a) {
+__host__ __device__ __forceinline__ long long part_rows(const Kv8Attn& a) {
+  if (a.fit) return static_cast<long long>(a.fit) * a.tile_rows;
   return static_cast<long long>(a.seqs.batch) * a.pages.heads * a.row_groups * a.chunks * a.tile_rows;
+}
+
+// Cutting the keys by the lengths.  A grid sized on the host has to be sized for the longest sequence that there may be:
+// lengths that differ, or a loose max_len, then leave it half empty.  Here every CTA looks at all lengths and finds the
+// smallest chunk (a multiple of 128 keys, a.chunk at the least) whose chunks are at most a.fit, and then which one is
+// its own: the chunks of a sequence follow one another, heads fastest.  Chunks are not the same length in all lengths'
+// calls, so neither are a sequence's roundings; the same lengths give the same bits.
+constexpr int kFitBatch = 512;  // sequences of a call with fit, at most
+// A sequence's cut, for the kernel that joins the chunks: its first CTA, its chunks (of each row group), their length,
+// and its row groups.
+__device__ __forceinline__ int4* cuts_of(const Kv8Attn& a) {
+  return reinterpret_cast<int4*>(a.part + part_rows(a) * (a.head_dim + 2));
+}
+// A quotient that rounding leaves one too high or too low does no harm: the last chunk takes what is left, and an empty
+// one ends at once.
+__device__ __forceinline__ int chunks_of(int span, float per_key) { return max(__float2int_ru(span * per_key), 1); }
+// The same value of every thread as one that the compiler knows to be: it stays in a uniform register.
+__device__ __forceinline__ int uniform(int x) { return static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<unsigned>(x))); }
+// The CTA's place; false: none is left for it.  memory: room for a.seqs.batch entries, used until this returns (and, by
+// the async proxy's clock, done with).  Every thread of the block takes part, warps beside one another do the same.
+__device__ __forceinline__ bool fit_place(const Kv8Attn& a, int cta, int2* memory, Place& p) {
+  const int lane = threadIdx.x & 31, n = a.seqs.batch;
+  // the keys that a row group of a sequence sees at the most, from a multiple of 32 on, and its CTAs of a chunk
+  auto look = [&](int b) {
+    long long row0;
+    const long long R = static_cast<long long>(seq_rows(a.seqs, b, row0)) * a.group;
+    const int groups = static_cast<int>(min(static_cast<long long>(a.row_groups), (R + a.tile_rows - 1) / a.tile_rows));
+    int span = seq_length(a, b);
+    if (a.window) span = min(span, min(a.window, 1 << 29) + a.tile_rows / a.group + 32);
+    return make_int2(span + 31, groups * a.pages.heads);
+  };
+  // the first 32 sequences are in registers, the others, where there are more, in memory
+  const int2 own = lane < n ? look(lane) : make_int2(0, 0);
+  if (n > 32) {
+#pragma unroll 1
+    for (int b = 32 + threadIdx.x; b < n; b += blockDim.x) memory[b] = look(b);
+    __syncthreads();
+  }
+  auto seq = [&](int b) { return b < 32 ? own : memory[b]; };  // b % 32 == lane
+  long long total = 0;
+  int longest = 0, items = 0;
+#pragma unroll 1
+  for (int b = lane; b < n; b += 32) {
+    const int2 s = seq(b);
+    total += static_cast<long long>(s.x) * s.y;
+    longest = max(longest, s.x), items += s.y;
+  }
+#pragma unroll 1
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  longest = uniform(longest);
+  items = __reduce_add_sync(0xffffffffu, items);
+  auto fits = [&](int tiles) {
+    const float per_key = __fdividef(1.0f, tiles * 128);
+    int sum = 0;
+#pragma unroll 1
+    for (int b = lane; b < n; b += 32) sum += chunks_of(seq(b).x, per_key) * seq(b).y;
+    return __reduce_add_sync(0xffffffffu, sum) <= a.fit;
+  };
+  // Chunks of total / fit keys are too many, except where nothing is left over.  Those of total / (fit - items) should be
+  // few enough, since an item has at most one chunk that is not full; those of the longest sequence are, as there are no
+  // more than fit items.
+  auto share = [&](int ctas) { return __float2int_rd(fminf(__fdividef(static_cast<float>(total), static_cast<float>(ctas)), 1e9f)); };
+  const int most = max(longest, a.chunk) / 128 + 1;
+  int lo = min(max(a.chunk, share(a.fit)) / 128, most), hi = items < a.fit ? max(min(share(a.fit - items) / 128 + 1, most), lo) : most;
+  int mid = hi;
+#pragma unroll 1
+  do {
+    if (fits(mid))
+      hi = mid;
+    else if (mid == hi)
+      lo = hi + 1, hi = most;  // the guess was too low
+    else
+      lo = mid + 1;
+    mid = (lo + hi) >> 1;
+  } while (lo < hi);
+  p.keys = uniform(hi * 128);
+  const float per_key = __fdividef(1.0f, p.keys);
+  bool there = false;
+  int before = 0;  // CTAs of the sequences so far
+#pragma unroll 1
+  for (int b0 = 0; b0 < n && !there; b0 += 32) {
+    const int2 s = b0 + lane < n ? seq(b0 + lane) : make_int2(0, 0);
+    const int mine = chunks_of(s.x, per_key) * s.y;
+    int upto = mine;
+#pragma unroll 1
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    upto += before;
+    const unsigned found = __ballot_sync(0xffffffffu, cta < upto);
+    if (found) {
+      const int at = __ffs(found) - 1;
+      const int first = uniform(__shfl_sync(0xffffffffu, upto - mine, at)), one = uniform(__shfl_sync(0xffffffffu, s.y, at));
+      p.b = uniform(b0 + at);
+      p.chunk = uniform((cta - first) / one);
+      const int item = cta - first - p.chunk * one, rg = uniform(item / a.pages.heads);
+      p.h = item - rg * a.pages.heads;
+      p.rg = one / a.pages.heads - 1 - rg;  // the longest (the last of a causal sequence) first
+      p.chunks = uniform(chunks_of(__shfl_sync(0xffffffffu, s.x, at), per_key));
+      p.part = static_cast<long long>(cta) * a.tile_rows;
+      if (cta == first && threadIdx.x == 0) cuts_of(a)[p.b] = make_int4(first, p.chunks, p.keys, one);
+      there = true;
+    }
+    before = __shfl_sync(0xffffffffu, upto, 31);
+  }
+  if (n > 32) {
+    fence_proxy_async_smem();
+    __syncthreads();
+  }
+  return there;
 }
 
 // mbar_wait for a whole warp: every lane goes on, or none does.
@@ -292,9 +412,8 @@ inline cudaError_t once_per_device(std::atomic<bool> (&done)[64], F set) {
   return r;
 }
 inline size_t kv8_part_bytes(const Kv8Attn& a) {
-  if (a.chunks <= 1) return 0;
-  return static_cast<size_t>(a.seqs.batch) * a.pages.heads * a.row_groups * a.chunks * a.tile_rows * (a.head_dim + 2) *
-         sizeof(float);
+  if (a.chunks <= 1 && a.fit == 0) return 0;
+  return static_cast<size_t>(kv8::part_rows(a)) * (a.head_dim + 2) * sizeof(float) + (a.fit ? a.seqs.batch * sizeof(int4) : 0);
 }
 
 }  // namespace qhtp

@@ -177,7 +177,7 @@ QhtpStatus qhtp_kv8_attention(const QhtpKv8Attention* run) {
   a.part = static_cast<float*>(run->workspace);
   a.stream = static_cast<cudaStream_t>(run->stream);
   cudaError_t e = a.prompt ? (a.tile_rows == 256 ? launch_kv8_prompt2(a) : launch_kv8_prompt(a)) : launch_kv8_decode(a);
-  if (e == cudaSuccess && a.chunks > 1) e = launch_kv8_combine(a);
+  if (e == cudaSuccess && (a.chunks > 1 || a.fit)) e = launch_kv8_combine(a);
   return status_from_cuda(e);
 }
 

@@ -68,7 +68,8 @@ struct Ring {
   static_assert(2 * 8 * NT * (D + 4) * 4 <= smem - 1024, "the rows are joined in the rings' memory");
 };
 
-template <int D, int NT>
+// FIT: cut by fit_place, else on the plan's grid.  Two kernels, since that code costs the other one registers.
+template <int D, int NT, bool FIT>
 __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 3)  // as many as the rings leave room for
     kv8_decode_kernel(const Kv8Attn a, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
   using Rg = Ring<D, NT>;
@@ -90,19 +91,28 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 3)  // as many as t
   float* const s_o = reinterpret_cast<float*>(ring);
   int* const err = &g_error;
 
-  // chunks slowest: the first ones, which every sequence has whole, run first, and the remainders fill the end
-  const int b = blockIdx.y, h = blockIdx.x / a.row_groups, rg = blockIdx.x - h * a.row_groups, chunk = blockIdx.z;
+  __shared__ Place s_place;  // for the end
+  Place at;
+  if constexpr (FIT) {
+    if (!fit_place(a, blockIdx.x, reinterpret_cast<int2*>(ring), at)) return;
+  } else {
+    // chunks slowest: the first ones, which every sequence has whole, run first, and the remainders fill the end
+    at.b = blockIdx.y, at.h = blockIdx.x / a.row_groups, at.rg = blockIdx.x - at.h * a.row_groups, at.chunk = blockIdx.z;
+    at.chunks = a.chunks, at.keys = a.chunk, at.part = part_row(a, at.b, at.h, at.rg, at.chunk);
+  }
+  const int b = at.b, h = at.h;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
   long long row0;
   const int T = seq_rows(a.seqs, b, row0);
-  const int R = T * a.group, r0 = rg * kRows;
+  const int R = T * a.group, r0 = at.rg * kRows;
   if (r0 >= R) return;
   const int r1 = min(R, r0 + kRows);
   const int len = seq_length(a, b);
   const Span all = row_span(a, len, T, r0, r1);
-  const Span keys = chunk_span(a, all, chunk);
+  const Span keys = chunk_span(at, all);
+  if (threadIdx.x == 0) s_place = at;
   // an empty chunk leaves nothing; where every chunk is empty, the first one writes the rows
-  if (keys.lo >= keys.hi && chunk > 0) return;
+  if (keys.lo >= keys.hi && at.chunk > 0) return;
   // each row of the group sees the keys [all_lo, all_hi)
   const int all_hi = a.causal ? len - T + r0 / a.group + 1 : len;
   const int all_lo = a.window ? len - T + (r1 - 1) / a.group - a.window + 1 : 0;
@@ -409,7 +419,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 3)  // as many as t
     __syncthreads();
   }
 
-  const long long part = part_row(a, b, h, rg, chunk);
+  const long long part = s_place.part;
+  const bool whole = s_place.chunks == 1;
   for (int i = threadIdx.x; i < kRows * (D / 8); i += kWarps * 32) {
     const int r = i / (D / 8), c = i - r * (D / 8), row = r0 + r;
     if (row >= r1) break;
@@ -427,7 +438,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 3)  // as many as t
 #pragma unroll
       for (int w = 0; w < kAreas; ++w) o[e] += s_o[w * kArea + r * kOStride + 8 * c + e];
     }
-    if (a.chunks == 1) {
+    if (whole) {
       write_row8(a, b, row0, row, h, 8 * c, o, sum, base);
     } else {
       float4* to = reinterpret_cast<float4*>(a.part + (part + r) * D + 8 * c);
@@ -441,48 +452,72 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 3)  // as many as t
   }
 }
 
-constexpr int kFew = 8;
-
-// Chunks that a row group's keys fill: those that its attention kernel wrote.
-__device__ __forceinline__ int chunks_used(const Kv8Attn& a, const Span& s) {
+// A row's parts: those that its attention kernel wrote, `step` rows apart.  None: the row is not there, or finished.
+struct Parts {
+  int b, h, row, n;
+  long long row0, first, step;
+  __device__ __forceinline__ long long at(int i) const { return first + i * step; }
+};
+__device__ __forceinline__ Parts parts_of(const Kv8Attn& a, int row) {
+  Parts p{static_cast<int>(blockIdx.z), static_cast<int>(blockIdx.y), row, 0};
+  const int T = seq_rows(a.seqs, p.b, p.row0);
+  const int R = T * a.group, rg = row / a.tile_rows, r0 = rg * a.tile_rows, r1 = min(R, r0 + a.tile_rows);
+  if (row >= R || rg >= a.row_groups) return p;
+  int chunks = a.chunks, keys = a.chunk;
+  if (a.fit) {
+    const int4 cut = cuts_of(a)[p.b];
+    if (cut.y == 1) return p;
+    chunks = cut.y, keys = cut.z;
+    p.first = static_cast<long long>(cut.x + cut.w - (rg + 1) * a.pages.heads + p.h) * a.tile_rows;
+    p.step = static_cast<long long>(cut.w) * a.tile_rows;
+  } else {
+    p.first = part_row(a, p.b, p.h, rg, 0);
+    p.step = a.tile_rows;
+  }
+  p.first += row - r0;
+  const Span s = row_span(a, seq_length(a, p.b), T, r0, r1);
   const long long span = s.hi - (s.lo & ~31);
-  return span <= 0 ? 1 : static_cast<int>(min(static_cast<long long>(a.chunks), (span + a.chunk - 1) / a.chunk));
+  p.n = span <= 0 ? 1 : static_cast<int>(min(static_cast<long long>(chunks), (span + keys - 1) / keys));
+  return p;
 }
 
-// The chunks of each row joined, few of them: D / 8 threads a row, each over all chunks.
+// The chunks of each row joined, few of them: D / 8 threads a row, each over all chunks, kFew at a time.
+constexpr int kFew = 8;
 template <int D>
 __global__ void __launch_bounds__(128) kv8_combine_few_kernel(const Kv8Attn a) {
   constexpr int kLanes = D / 8, kPer = 128 / kLanes;
   griddep_wait();
-  const int b = blockIdx.z, h = blockIdx.y, row = blockIdx.x * kPer + threadIdx.x / kLanes, c = threadIdx.x % kLanes;
-  long long row0;
-  const int T = seq_rows(a.seqs, b, row0);
-  const int R = T * a.group, rg = row / a.tile_rows, r0 = rg * a.tile_rows, r1 = min(R, r0 + a.tile_rows), r = row - r0;
-  if (row >= R || rg >= a.row_groups) return;
-  const int n = chunks_used(a, row_span(a, seq_length(a, b), T, r0, r1));
-  const long long part = part_row(a, b, h, rg, 0) + r;
+  const int c = threadIdx.x % kLanes;
+  const Parts p = parts_of(a, blockIdx.x * kPer + threadIdx.x / kLanes);
+  if (p.n == 0) return;
   const float* const ml = a.part + part_rows(a) * D;
-  float top = -INFINITY, l[kFew], m[kFew];
+  float top = -INFINITY, sum = 0.0f, o[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i0 = 0; i0 < p.n; i0 += kFew) {
+    float l[kFew], m[kFew];
+    const float before = top;
 #pragma unroll
-  for (int i = 0; i < kFew; ++i) {
-    const float2 v = i < n ? *reinterpret_cast<const float2*>(ml + 2 * (part + static_cast<long long>(i) * a.tile_rows))
-                           : make_float2(0.0f, 0.0f);
-    m[i] = v.x, l[i] = v.y;
-    if (v.y != 0.0f) top = fmaxf(top, v.x);
-  }
-  if (top == -INFINITY) top = 0.0f;
-  float sum = 0.0f, o[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < kFew; ++i) {
+      const float2 v = i0 + i < p.n ? *reinterpret_cast<const float2*>(ml + 2 * p.at(i0 + i)) : make_float2(0.0f, 0.0f);
+      m[i] = v.x, l[i] = v.y;
+      if (v.y != 0.0f) top = fmaxf(top, v.x);
+    }
+    if (top == -INFINITY) continue;  // no key yet
+    const float alpha = ex2(before - top);
+    sum *= alpha;
 #pragma unroll
-  for (int i = 0; i < kFew; ++i) {
-    if (i >= n) break;
-    const float4* x = reinterpret_cast<const float4*>(a.part + (part + static_cast<long long>(i) * a.tile_rows) * D + 8 * c);
-    const float4 u = x[0], v = x[1];
-    const float f = l[i] != 0.0f ? ex2(m[i] - top) : 0.0f;
-    sum = fmaf(l[i], f, sum);
-    o[0] = fmaf(u.x, f, o[0]), o[1] = fmaf(u.y, f, o[1]), o[2] = fmaf(u.z, f, o[2]), o[3] = fmaf(u.w, f, o[3]);
-    o[4] = fmaf(v.x, f, o[4]), o[5] = fmaf(v.y, f, o[5]), o[6] = fmaf(v.z, f, o[6]), o[7] = fmaf(v.w, f, o[7]);
+    for (int e = 0; e < 8; ++e) o[e] *= alpha;
+#pragma unroll
+    for (int i = 0; i < kFew; ++i) {
+      if (i0 + i >= p.n) break;
+      const float4* x = reinterpret_cast<const float4*>(a.part + p.at(i0 + i) * D + 8 * c);
+      const float4 u = x[0], v = x[1];
+      const float f = l[i] != 0.0f ? ex2(m[i] - top) : 0.0f;
+      sum = fmaf(l[i], f, sum);
+      o[0] = fmaf(u.x, f, o[0]), o[1] = fmaf(u.y, f, o[1]), o[2] = fmaf(u.z, f, o[2]), o[3] = fmaf(u.w, f, o[3]);
+      o[4] = fmaf(v.x, f, o[4]), o[5] = fmaf(v.y, f, o[5]), o[6] = fmaf(v.z, f, o[6]), o[7] = fmaf(v.w, f, o[7]);
+    }
   }
-  write_row8(a, b, row0, row, h, 8 * c, o, sum, top);
+  write_row8(a, p.b, p.row0, p.row, p.h, 8 * c, o, sum, top == -INFINITY ? 0.0f : top);
 }
 
 // The chunks of a row joined: a CTA a row.  Its threads take the chunks' maxima and sums at once, then each eight
@@ -493,19 +528,15 @@ __global__ void __launch_bounds__(256) kv8_combine_kernel(const Kv8Attn a) {
   __shared__ float s_w[kWeights], s_top[8], s_sum[8];
   __shared__ float s_o[kGroups][D + 4];
   griddep_wait();
-  const int b = blockIdx.z, h = blockIdx.y, row = blockIdx.x, t = threadIdx.x;
-  long long row0;
-  const int T = seq_rows(a.seqs, b, row0);
-  const int R = T * a.group, rg = row / a.tile_rows, r0 = rg * a.tile_rows, r1 = min(R, r0 + a.tile_rows), r = row - r0;
-  if (row >= R || rg >= a.row_groups) return;
-  const int n = chunks_used(a, row_span(a, seq_length(a, b), T, r0, r1));
-  const long long part = part_row(a, b, h, rg, 0) + r;
+  const int t = threadIdx.x;
+  const Parts p = parts_of(a, blockIdx.x);
+  const int n = p.n;
+  if (n == 0) return;
   const float* const ml = a.part + part_rows(a) * D;
-  auto at = [&](int i) { return part + static_cast<long long>(i) * a.tile_rows; };
   // the row's maximum over the chunks that saw a key of it
   float top = -INFINITY;
   for (int i = t; i < n; i += 256) {
-    const float2 v = *reinterpret_cast<const float2*>(ml + 2 * at(i));
+    const float2 v = *reinterpret_cast<const float2*>(ml + 2 * p.at(i));
     if (v.y != 0.0f) top = fmaxf(top, v.x);
   }
 #pragma unroll
@@ -521,7 +552,7 @@ __global__ void __launch_bounds__(256) kv8_combine_kernel(const Kv8Attn a) {
   for (int base = 0; base < n; base += kWeights) {
     const int m = min(kWeights, n - base);
     if (t < m) {
-      const float2 v = *reinterpret_cast<const float2*>(ml + 2 * at(base + t));
+      const float2 v = *reinterpret_cast<const float2*>(ml + 2 * p.at(base + t));
       const float w = v.y != 0.0f ? ex2(v.x - top) : 0.0f;
       s_w[t] = w;
       sum = fmaf(v.y, w, sum);
@@ -529,7 +560,7 @@ __global__ void __launch_bounds__(256) kv8_combine_kernel(const Kv8Attn a) {
     __syncthreads();
 #pragma unroll 4
     for (int i = group; i < m; i += kGroups) {
-      const float4* x = reinterpret_cast<const float4*>(a.part + at(base + i) * D + 8 * c);
+      const float4* x = reinterpret_cast<const float4*>(a.part + p.at(base + i) * D + 8 * c);
       const float4 u = x[0], v = x[1];
       const float f = s_w[i];
       o[0] = fmaf(u.x, f, o[0]), o[1] = fmaf(u.y, f, o[1]), o[2] = fmaf(u.z, f, o[2]), o[3] = fmaf(u.w, f, o[3]);
@@ -552,11 +583,11 @@ __global__ void __launch_bounds__(256) kv8_combine_kernel(const Kv8Attn a) {
     o[e] = 0.0f;
     for (int i = 0; i < kGroups; ++i) o[e] += s_o[i][8 * t + e];
   }
-  write_row8(a, b, row0, row, h, 8 * t, o, sum, top);
+  write_row8(a, p.b, p.row0, p.row, p.h, 8 * t, o, sum, top);
 }
 
-template <int D, int NT>
-cudaError_t run(const Kv8Attn& a) {
+template <int D, int NT, bool FIT>
+cudaError_t run_as(const Kv8Attn& a) {
   using Rg = Ring<D, NT>;
   CUtensorMap map[2];
   const uint64_t tiles = static_cast<uint64_t>(a.pages.num_blocks) * a.pages.heads;
@@ -566,12 +597,17 @@ cudaError_t run(const Kv8Attn& a) {
       return cudaErrorInvalidValue;
   static std::atomic<bool> done[64];
   const cudaError_t e = once_per_device(done, [] {
-    return cudaFuncSetAttribute(kv8_decode_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Rg::smem);
+    return cudaFuncSetAttribute(kv8_decode_kernel<D, NT, FIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Rg::smem);
   });
   if (e != cudaSuccess) return e;
-  const dim3 grid(static_cast<unsigned>(a.pages.heads) * a.row_groups, a.seqs.batch, a.chunks);
-  kv8_decode_kernel<D, NT><<<grid, kWarps * 32, Rg::smem, a.stream>>>(a, map[0], map[1]);
+  const dim3 grid = FIT ? dim3(a.fit) : dim3(static_cast<unsigned>(a.pages.heads) * a.row_groups, a.seqs.batch, a.chunks);
+  kv8_decode_kernel<D, NT, FIT><<<grid, kWarps * 32, Rg::smem, a.stream>>>(a, map[0], map[1]);
   return cudaGetLastError();
+}
+
+template <int D, int NT>
+cudaError_t run(const Kv8Attn& a) {
+  return a.fit ? run_as<D, NT, true>(a) : run_as<D, NT, false>(a);
 }
 
 template <int D>
@@ -614,6 +650,12 @@ void kv8_decode_plan(Kv8Attn& a, int sms) {
   if (span > kWhole) {
     n = (span + kMost - 1) / kMost;
     if (n * tiles < 4 * slots) n = std::max(1ll, std::min(slots / tiles, span / kLeast));
+    if (n * tiles <= slots && a.seqs.batch <= kv8::kFitBatch) {
+      a.fit = static_cast<int>(slots);
+      a.chunk = kLeast;
+      a.chunks = static_cast<int>(n);
+      return;
+    }
   }
   n = std::min(n, 65535ll);  // grid.z
   const long long chunk = ((span + n - 1) / n + 127) / 128 * 128;

@@ -38,6 +38,7 @@ struct Small {
   float half[2][2][128];
   Barriers bar;
   uint32_t tmem;
+  Place place;            // for the end: what the block is about takes no registers until then
 };
 
 template <int D>
@@ -65,7 +66,8 @@ struct Shape {
 
 __device__ int g_error;  // a wait that gave up leaves its code here
 
-template <int D>
+// FIT: cut by fit_place, else on the plan's grid.  Two kernels, since that code costs the other one registers.
+template <int D, bool FIT>
 __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const Kv8Attn a) {
   using S = Shape<D>;
   int* const err = &g_error;
@@ -77,19 +79,27 @@ __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const 
   float4(&s_scale)[8][4] = small.scale;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // heads fastest, the longest row groups (the last of a causal sequence) first
-  const int h = blockIdx.x / a.chunks, chunk = blockIdx.x - h * a.chunks, b = blockIdx.y,
-            rg = a.row_groups - 1 - blockIdx.z;
+  Place place;
+  if constexpr (FIT) {
+    if (!fit_place(a, blockIdx.x, reinterpret_cast<int2*>(smem), place)) return;
+  } else {
+    // heads fastest, the longest row groups (the last of a causal sequence) first
+    place.h = blockIdx.x / a.chunks, place.chunk = blockIdx.x - place.h * a.chunks, place.b = blockIdx.y;
+    place.rg = a.row_groups - 1 - blockIdx.z;
+    place.chunks = a.chunks, place.keys = a.chunk, place.part = part_row(a, place.b, place.h, place.rg, place.chunk);
+  }
+  const int b = place.b, h = place.h;
   long long row0;
   const int T = seq_rows(a.seqs, b, row0);
-  const int R = T * a.group, r0 = rg * 128;
+  const int R = T * a.group, r0 = place.rg * 128;
   if (r0 >= R) return;
   const int r1 = min(R, r0 + 128);
   const int len = seq_length(a, b);
   const Span all = row_span(a, len, T, r0, r1);
-  const Span keys = chunk_span(a, all, chunk);
+  const Span keys = chunk_span(place, all);
+  if (threadIdx.x == 0) small.place = place;
   const int units = keys.lo < keys.hi ? (keys.hi - keys.lo + kKeys - 1) / kKeys : 0;
-  if (units == 0 && chunk > 0) return;
+  if (units == 0 && place.chunk > 0) return;
 
   uint8_t* const k_img = smem + S::q_smem;
   uint8_t* const v_img = k_img + S::k_units * S::unit;
@@ -210,13 +220,13 @@ __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const 
     l = s_half[units & 1][0][in_tile] + s_half[units & 1][1][in_tile];
     const float base = m == -INFINITY ? 0.0f : m;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const long long part0 = part_row(a, b, h, rg, chunk) + wq * 32, part = part0 + lane;
+    const long long part0 = small.place.part + wq * 32, part = part0 + lane;
     // K's images are free: every S has been computed.  Rows of head_dim 64 are one piece, which the first half's warp takes.
     if (D > 64 || half == 0)
       rows_out<D, (D > 64 ? D / 2 : 64)>(a, b, h, row0, r0 + wq * 32, r1, part0, units == 0, o_at, D > 64 ? half * (D / 2) : 0, inv,
-                                         smem_u32(k_img) + warp * 4096, lane);
+                                         small.place.chunks == 1, smem_u32(k_img) + warp * 4096, lane);
     const bool live = r < r1 && half == 0;
-    if (live && a.chunks > 1) {
+    if (live && small.place.chunks > 1) {
       float* ml = a.part + part_rows(a) * D + 2 * part;
       ml[0] = base, ml[1] = l;
     } else if (live && a.lse != nullptr) {
@@ -366,27 +376,32 @@ __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const 
   if (warp == kMma) tmem_dealloc(tmem, 512);
 }
 
-template <int D>
+template <int D, bool FIT>
 cudaError_t prepare() {
   using S = Shape<D>;
-  cudaError_t e = cudaFuncSetAttribute(kv8_prompt_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem);
+  cudaError_t e = cudaFuncSetAttribute(kv8_prompt_kernel<D, FIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem);
   if (e != cudaSuccess) return e;
   cudaFuncAttributes at;
-  if ((e = cudaFuncGetAttributes(&at, kv8_prompt_kernel<D>)) != cudaSuccess) return e;
+  if ((e = cudaFuncGetAttributes(&at, kv8_prompt_kernel<D, FIT>)) != cudaSuccess) return e;
   // the roles' registers come out of what the launch has: more than that would be waited for without end
   if (at.numRegs != S::regs) return cudaErrorInvalidConfiguration;
   return cudaSuccess;
 }
 
-template <int D>
-cudaError_t run(const Kv8Attn& a) {
+template <int D, bool FIT>
+cudaError_t run_as(const Kv8Attn& a) {
   using S = Shape<D>;
   static std::atomic<bool> done[64];
-  const cudaError_t e = once_per_device(done, prepare<D>);
+  const cudaError_t e = once_per_device(done, prepare<D, FIT>);
   if (e != cudaSuccess) return e;
-  const dim3 grid(static_cast<unsigned>(a.pages.heads) * a.chunks, a.seqs.batch, a.row_groups);
-  kv8_prompt_kernel<D><<<grid, S::threads, S::smem, a.stream>>>(a);
+  const dim3 grid = FIT ? dim3(a.fit) : dim3(static_cast<unsigned>(a.pages.heads) * a.chunks, a.seqs.batch, a.row_groups);
+  kv8_prompt_kernel<D, FIT><<<grid, S::threads, S::smem, a.stream>>>(a);
   return cudaGetLastError();
+}
+
+template <int D>
+cudaError_t run(const Kv8Attn& a) {
+  return a.fit ? run_as<D, true>(a) : run_as<D, false>(a);
 }
 
 }  // namespace
@@ -396,15 +411,26 @@ void kv8_prompt_plan(Kv8Attn& a, int sms) {
   const long long rows = static_cast<long long>(a.seqs.tokens) * a.group;
   a.tile_rows = a.head_dim == 256 || rows <= 128 ? 128 : 256;
   a.row_groups = static_cast<int>((rows + a.tile_rows - 1) / a.tile_rows);
-  const long long tiles = static_cast<long long>(a.seqs.batch) * a.pages.heads * a.row_groups;
+  // row groups of all sequences: the most that there can be, and about how many
+  const long long most = static_cast<long long>(a.seqs.batch) * a.row_groups;
+  const long long about = a.seqs.start ? std::min(most, a.seqs.total * a.group / a.tile_rows + (a.seqs.batch + 1) / 2) : most;
   long long span = a.max_len;
   if (a.window) span = std::min(span, static_cast<long long>(a.window) + a.tile_rows / a.group + 32);
   span = std::max(span, 1ll);
-  // where the row groups do not fill the SMs, the keys are cut, into 512 at the least
-  const long long want = std::max(1ll, std::min(sms / tiles, span / 512));
-  const long long chunk = ((span + want - 1) / want + 127) / 128 * 128;
-  a.chunk = static_cast<int>(chunk);
-  a.chunks = static_cast<int>((span + chunk - 1) / chunk);
+  a.chunks = 1;
+  a.chunk = static_cast<int>((span + 127) / 128 * 128);
+  constexpr long long kLeast = 512;
+  if (span < 2 * kLeast) return;
+  const long long tiles = about * a.pages.heads;
+  if (2 * most * a.pages.heads <= sms && a.seqs.batch <= kv8::kFitBatch) {
+    a.fit = sms;
+    a.chunk = kLeast;
+    a.chunks = static_cast<int>(std::min(sms / (most * a.pages.heads), span / kLeast));
+  } else if (span >= 4096 && tiles > sms && 2 * tiles <= 3 * sms) {
+    // three waves of half the keys are less than two of all
+    a.chunk = static_cast<int>((span / 2 + 127) / 128 * 128);
+    a.chunks = 2;
+  }
 }
 
 cudaError_t launch_kv8_prompt(const Kv8Attn& a) {

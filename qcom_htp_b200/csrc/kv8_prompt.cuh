@@ -193,10 +193,9 @@ struct RowsOut {
 // are to the parts.  rw: the warp's first row of the group; part0: its part.
 template <int D, int COLS>
 __device__ __forceinline__ void rows_out(const Kv8Attn& a, int b, int h, long long row0, int rw, int r1, long long part0, bool zero,
-                                         uint32_t o_at, int col0, float inv, uint32_t stage, int lane) {
+                                         uint32_t o_at, int col0, float inv, bool whole, uint32_t stage, int lane) {
   RowsOut o;
   o.stage = stage;
-  const bool whole = a.chunks == 1;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     const int i = 4 * k + (lane >> 3), r = rw + i, t = r / a.group, head = h * a.group + r - t * a.group;

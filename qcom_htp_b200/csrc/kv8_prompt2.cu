@@ -40,32 +40,42 @@ struct Barriers2 {
 
 __device__ int g_error2;  // a wait that gave up leaves its code here
 
-template <int D>
+// FIT: cut by fit_place, else on the plan's grid.  Two kernels, since that code costs the other one registers.
+template <int D, bool FIT>
 __global__ void __launch_bounds__(Shape2<D>::threads, 1) kv8_prompt2_kernel(const Kv8Attn a) {
   using S = Shape2<D>;
   int* const err = &g_error2;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Barriers2 bar;
   __shared__ uint32_t s_tmem;
+  __shared__ Place s_place;  // for the end: what the block is about takes no registers until then
   __shared__ float s_down[256];
   __shared__ float s_half[2][2][2][128];  // [turn][slot][half][row]: a half row's maximum, at the end its sum
   __shared__ float4 s_scale[4][8];        // (c, log2 w, 1 / w, care) of a tile's 16-key groups, four tiles deep
-  static_assert(sizeof(Barriers2) + 1024 + 4096 + 512 + 4 + S::smem <= 227 * 1024, "shared memory");
+  static_assert(sizeof(Barriers2) + 1024 + 4096 + 512 + 4 + sizeof(Place) + S::smem <= 227 * 1024, "shared memory");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // heads fastest, the longest row groups (the last of a causal sequence) first
-  const int h = blockIdx.x / a.chunks, chunk = blockIdx.x - h * a.chunks, b = blockIdx.y,
-            rg = a.row_groups - 1 - blockIdx.z;
+  Place place;
+  if constexpr (FIT) {
+    if (!fit_place(a, blockIdx.x, reinterpret_cast<int2*>(smem_raw), place)) return;
+  } else {
+    // heads fastest, the longest row groups (the last of a causal sequence) first
+    place.h = blockIdx.x / a.chunks, place.chunk = blockIdx.x - place.h * a.chunks, place.b = blockIdx.y;
+    place.rg = a.row_groups - 1 - blockIdx.z;
+    place.chunks = a.chunks, place.keys = a.chunk, place.part = part_row(a, place.b, place.h, place.rg, place.chunk);
+  }
+  const int b = place.b, h = place.h;
   long long row0;
   const int T = seq_rows(a.seqs, b, row0);
-  const int R = T * a.group, r0 = rg * 256;
+  const int R = T * a.group, r0 = place.rg * 256;
   if (r0 >= R) return;
   const int r1 = min(R, r0 + 256);
   const int len = seq_length(a, b);
   const Span all = row_span(a, len, T, r0, r1);
-  const Span keys = chunk_span(a, all, chunk);
+  const Span keys = chunk_span(place, all);
+  if (threadIdx.x == 0) s_place = place;
   const int tiles = keys.lo < keys.hi ? (keys.hi - keys.lo + kTile - 1) / kTile : 0;
-  if (tiles == 0 && chunk > 0) return;
+  if (tiles == 0 && place.chunk > 0) return;
 
   uint8_t* const q_img = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint8_t* const k_img = q_img + 2 * S::q_tile;
@@ -197,15 +207,15 @@ __global__ void __launch_bounds__(Shape2<D>::threads, 1) kv8_prompt2_kernel(cons
       const float base = m == -INFINITY ? 0.0f : m;
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       const int rw = sr0 + wq * 32;
-      const long long part0 = part_row(a, b, h, rg, chunk) + slot * 128 + wq * 32, part = part0 + lane;
+      const long long part0 = s_place.part + slot * 128 + wq * 32, part = part0 + lane;
       // K's images are free: every S has been computed.  Rows of
       // head_dim 64 are one piece, which the first half's warp takes.
       if (D == 128 || half == 0)
-        rows_out<D, 64>(a, b, h, row0, rw, sr1, part0, tiles == 0, o_at, half * 64, inv,
+        rows_out<D, 64>(a, b, h, row0, rw, sr1, part0, tiles == 0, o_at, half * 64, inv, s_place.chunks == 1,
                         smem_u32(k_img) + (D == 128 ? warp : slot * 4 + wq) * 4096, lane);
       const bool live = r < sr1;
       if (half == 0 && live) {
-        if (a.chunks > 1) {
+        if (s_place.chunks > 1) {
           float* ml = a.part + part_rows(a) * D + 2 * part;
           ml[0] = base, ml[1] = l;
         } else if (a.lse != nullptr) {
@@ -357,26 +367,31 @@ __global__ void __launch_bounds__(Shape2<D>::threads, 1) kv8_prompt2_kernel(cons
   if (warp == kMma) tmem_dealloc(tmem, 512);
 }
 
-template <int D>
+template <int D, bool FIT>
 cudaError_t prepare2() {
   using S = Shape2<D>;
-  cudaError_t e = cudaFuncSetAttribute(kv8_prompt2_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem);
+  cudaError_t e = cudaFuncSetAttribute(kv8_prompt2_kernel<D, FIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem);
   if (e != cudaSuccess) return e;
   cudaFuncAttributes at;
-  if ((e = cudaFuncGetAttributes(&at, kv8_prompt2_kernel<D>)) != cudaSuccess) return e;
+  if ((e = cudaFuncGetAttributes(&at, kv8_prompt2_kernel<D, FIT>)) != cudaSuccess) return e;
   // the roles' registers come out of what the launch has: more than that would be waited for without end
   return at.numRegs == S::regs ? cudaSuccess : cudaErrorInvalidConfiguration;
 }
 
-template <int D>
-cudaError_t run2(const Kv8Attn& a) {
+template <int D, bool FIT>
+cudaError_t run_as2(const Kv8Attn& a) {
   using S = Shape2<D>;
   static std::atomic<bool> done[64];
-  const cudaError_t e = once_per_device(done, prepare2<D>);
+  const cudaError_t e = once_per_device(done, prepare2<D, FIT>);
   if (e != cudaSuccess) return e;
-  const dim3 grid(static_cast<unsigned>(a.pages.heads) * a.chunks, a.seqs.batch, a.row_groups);
-  kv8_prompt2_kernel<D><<<grid, S::threads, S::smem, a.stream>>>(a);
+  const dim3 grid = FIT ? dim3(a.fit) : dim3(static_cast<unsigned>(a.pages.heads) * a.chunks, a.seqs.batch, a.row_groups);
+  kv8_prompt2_kernel<D, FIT><<<grid, S::threads, S::smem, a.stream>>>(a);
   return cudaGetLastError();
+}
+
+template <int D>
+cudaError_t run2(const Kv8Attn& a) {
+  return a.fit ? run_as2<D, true>(a) : run_as2<D, false>(a);
 }
 
 }  // namespace
