@@ -19,6 +19,13 @@ output, and turns a non-OK status into ``QhtpError`` (a ``RuntimeError``) carryi
     torch.ops.qhtp.gdn_inverse(A bf16 [..., C, C]) -> T float32
     torch.ops.qhtp.gdn_chunk_inverse(k bf16 [..., 256, 128], beta, g float32 [..., 256]) -> T float32
     torch.ops.qhtp.gdn_solve_u16(A uint16 [..., C, C], zpA, sA, zpT, sT) -> T uint16
+    torch.ops.qhtp.kv8_write(cache_k, cache_v, k_scale, v_scale, k, v, block_table, past,
+                             seq_start=None, max_new=None) -> None: changes the four cache tensors
+    torch.ops.qhtp.kv8_read(cache_k, cache_v, k_scale, v_scale, block_table, first, tokens=None, seq_start=None,
+                            total=None, max_tokens=None, dtype=bfloat16) -> (k, v)
+    torch.ops.qhtp.kv8_attention(q, cache_k, cache_v, k_scale, v_scale, block_table, lengths, scale=None, causal=True,
+                                 window=0, seq_start=None, max_new=None, max_len=None) -> (out, lse)
+        the 8-bit paged KV cache (qcom_htp_b200.kv8), with its tensors one by one.
 """
 from __future__ import annotations
 
@@ -27,6 +34,7 @@ from collections import OrderedDict
 import torch
 
 from . import gdn as _gdn
+from . import kv8 as _kv8
 from .matmul import FAMILY_BITS, QuantMatMul
 
 _CACHE: OrderedDict = OrderedDict()
@@ -137,3 +145,47 @@ def gdn_solve_u16_op(A: torch.Tensor, zpA: int, sA: float, zpT: int, sT: float) 
 @gdn_solve_u16_op.register_fake
 def _(A, zpA, sA, zpT, sT):
     return A.new_empty(A.shape, dtype=torch.uint16)
+
+
+@torch.library.custom_op("qhtp::kv8_write", mutates_args=("cache_k", "cache_v", "k_scale", "v_scale"), device_types="cuda")
+def kv8_write_op(cache_k: torch.Tensor, cache_v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                 k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, past: torch.Tensor,
+                 seq_start: torch.Tensor | None = None, max_new: int | None = None) -> None:
+    _kv8.kv8_write((cache_k, cache_v, k_scale, v_scale), k, v, block_table, past, seq_start=seq_start, max_new=max_new)
+
+
+@kv8_write_op.register_fake
+def _(cache_k, cache_v, k_scale, v_scale, k, v, block_table, past, seq_start=None, max_new=None):
+    return None
+
+
+@torch.library.custom_op("qhtp::kv8_read", mutates_args=(), device_types="cuda")
+def kv8_read_op(cache_k: torch.Tensor, cache_v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                block_table: torch.Tensor, first: torch.Tensor, tokens: int | None = None,
+                seq_start: torch.Tensor | None = None, total: int | None = None, max_tokens: int | None = None,
+                dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+    return _kv8.kv8_read((cache_k, cache_v, k_scale, v_scale), block_table, first, tokens, seq_start=seq_start, total=total,
+                         max_tokens=max_tokens, dtype=dtype)
+
+
+@kv8_read_op.register_fake
+def _(cache_k, cache_v, k_scale, v_scale, block_table, first, tokens=None, seq_start=None, total=None, max_tokens=None,
+      dtype=torch.bfloat16):
+    rows = (block_table.shape[0], tokens) if seq_start is None else (total,)
+    shape = (*rows, cache_k.shape[1], cache_k.shape[3])
+    return cache_k.new_empty(shape, dtype=dtype), cache_k.new_empty(shape, dtype=dtype)
+
+
+@torch.library.custom_op("qhtp::kv8_attention", mutates_args=(), device_types="cuda")
+def kv8_attention_op(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, k_scale: torch.Tensor,
+                     v_scale: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, scale: float | None = None,
+                     causal: bool = True, window: int = 0, seq_start: torch.Tensor | None = None,
+                     max_new: int | None = None, max_len: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    return _kv8.kv8_attention(q, (cache_k, cache_v, k_scale, v_scale), block_table, lengths, scale=scale, causal=causal,
+                              window=window, seq_start=seq_start, max_new=max_new, max_len=max_len, return_lse=True)
+
+
+@kv8_attention_op.register_fake
+def _(q, cache_k, cache_v, k_scale, v_scale, block_table, lengths, scale=None, causal=True, window=0, seq_start=None,
+      max_new=None, max_len=None):
+    return torch.empty_like(q), q.new_empty(q.shape[:-1], dtype=torch.float32)
