@@ -644,7 +644,7 @@ void kv8_decode_plan(Kv8Attn& a, int sms) {
   // sequences of unlike lengths to share the SMs.  Else the keys are cut so that the CTAs are one whole wave.  Short
   // spans are left whole: a CTA takes 512 keys in less time than a second kernel needs to join two parts.
   // Measured, 2 x 131072 keys: one wave 95.6 us, two 103.2, three 109.3, chunks of 2048 keys (2.3 waves) 110.
-  constexpr long long kMost = 2048, kLeast = 256, kWhole = 768;
+  constexpr long long kMost = 2048, kLeast = 128, kWhole = 768;
   const long long slots = 3ll * sms;
   long long n = 1;
   if (span > kWhole) {
