@@ -409,7 +409,7 @@ typedef struct QhtpKv8Attention {
   uint32_t dtype, q_heads;
   uint32_t causal, window;
   float scale;                /* finite, > 0 */
-  uint32_t max_len;           /* about the largest length: sizes the grid, changes no result */
+  uint32_t max_len;           /* about the largest length: sizes the launch; any value gives a right result */
   void *workspace;            /* qhtp_kv8_attention_workspace_bytes; 256-byte aligned */
   size_t workspace_bytes;
   void *stream;

@@ -210,8 +210,9 @@ __host__ __device__ __forceinline__ long long part_rows(const Kv8Attn& a) {
 // Cutting the keys by the lengths.  A grid sized on the host has to be sized for the longest sequence that there may be:
 // lengths that differ, or a loose max_len, then leave it half empty.  Here every CTA looks at all lengths and finds the
 // smallest chunk (a multiple of 128 keys, a.chunk at the least) whose chunks are at most a.fit, and then which one is
-// its own: the chunks of a sequence follow one another, heads fastest.  Chunks are not the same length in all lengths'
-// calls, so neither are a sequence's roundings; the same lengths give the same bits.
+// its own: the chunks of a sequence follow one another, heads fastest.  It costs a CTA some 3 us of its start (measured figures
+// are at the plans).  The cut, and with it a sequence's roundings, depends on all lengths of the call; the same lengths give
+// the same bits.
 constexpr int kFitBatch = 512;  // sequences of a call with fit, at most
 // A sequence's cut, for the kernel that joins the chunks: its first CTA, its chunks (of each row group), their length,
 // and its row groups.
@@ -266,9 +267,12 @@ __device__ __forceinline__ bool fit_place(const Kv8Attn& a, int cta, int2* memor
   // Chunks of total / fit keys are too many, except where nothing is left over.  Those of total / (fit - items) should be
   // few enough, since an item has at most one chunk that is not full; those of the longest sequence are, as there are no
   // more than fit items.
-  auto share = [&](int ctas) { return __float2int_rd(fminf(__fdividef(static_cast<float>(total), static_cast<float>(ctas)), 1e9f)); };
+  auto share = [&](int ctas) {
+    return __float2int_rd(fminf(__fdividef(static_cast<float>(total), static_cast<float>(ctas)), 1e9f));
+  };
   const int most = max(longest, a.chunk) / 128 + 1;
-  int lo = min(max(a.chunk, share(a.fit)) / 128, most), hi = items < a.fit ? max(min(share(a.fit - items) / 128 + 1, most), lo) : most;
+  int lo = min(max(a.chunk, share(a.fit)) / 128, most);
+  int hi = items < a.fit ? max(min(share(a.fit - items) / 128 + 1, most), lo) : most;
   int mid = hi;
 #pragma unroll 1
   do {

@@ -10,6 +10,9 @@
 // Bound by memory: two bytes per key and element.  The keys of a (sequence, kv head) are cut into chunks
 // over the grid, a CTA's four warps take 32 of them (16 at head_dim 256) in turn, and each warp keeps a ring of
 // them in shared memory filled by TMA, so that the loads in flight do not hang on registers or on what the warp does.
+// Measured: 2 sequences of 131072 keys, 8 kv heads x 128, 90 us (6.0 TB/s; 6.4 to 6.5 between the first loads and the last);
+// 64 of 4000 on average 101 us (5.3 TB/s); 16 of 9500 on average, 2 x 256, 35 us (4.4 TB/s).  What is left is a CTA's start
+// (some 4 us until its first keys arrive) and the last CTAs' end, and the join (3 to 5 us).
 // Keys are the M side of the MMAs (m16n8k16, S^T = K Q^T and O^T = V^T P^T), so a group of eight query rows
 // wastes nothing.  Which head_dim index a fragment's k stands for is free: a thread's 16 bytes of a key are its
 // fragments, and with the swizzle that TMA applies neither K's nor V's reads have bank conflicts (V of head_dim 64: two ways).
@@ -481,7 +484,9 @@ __device__ __forceinline__ Parts parts_of(const Kv8Attn& a, int row) {
   return p;
 }
 
-// The chunks of each row joined, few of them: D / 8 threads a row, each over all chunks, kFew at a time.
+// The chunks of each row joined, few of them: D / 8 threads a row, each over all chunks, kFew at a time.  Up to kFew chunks
+// (as many as equal lengths would have), else the kernel below: 2688 rows of 2 chunks 33.1 us with their attention, 41.3 by a CTA
+// a row; 64 rows of 27 chunks 98.2 by a CTA a row, 103.9 by this one.
 constexpr int kFew = 8;
 template <int D>
 __global__ void __launch_bounds__(128) kv8_combine_few_kernel(const Kv8Attn a) {
@@ -641,9 +646,14 @@ void kv8_decode_plan(Kv8Attn& a, int sms) {
   if (a.window) span = std::min(span, static_cast<long long>(a.window) + a.tile_rows + 31);
   span = std::max(span, 1ll);
   // Three CTAs fit an SM.  Where the row groups alone are many waves of those, chunks of kMost keys are short enough for
-  // sequences of unlike lengths to share the SMs.  Else the keys are cut so that the CTAs are one whole wave.  Short
-  // spans are left whole: a CTA takes 512 keys in less time than a second kernel needs to join two parts.
+  // sequences of unlike lengths to share the SMs.  Else the keys are cut so that the CTAs are one whole wave (by the lengths:
+  // fit_place).  Short spans are left whole: a CTA takes 512 keys in less time than a second kernel needs to join two parts.
   // Measured, 2 x 131072 keys: one wave 95.6 us, two 103.2, three 109.3, chunks of 2048 keys (2.3 waves) 110.
+  // 500 keys whole 10.5 us, in two 13.2; 1500 keys in chunks of 128 12.7 us, of 256 14.7, whole 18.7.
+  // By the lengths against chunks of the longest one's: 16 x up to 16000 keys of head_dim 256 42.4 us against 51.4, 24 x up to
+  // 12000 of head_dim 64 31.4 against 41.4; all lengths alike, 16 x 8000, 57.1 against 54.5: what finding its place costs a CTA.
+  // With more row groups than a wave holds: 64 x up to 8000 keys 108 us in chunks of 2048, 114 to 120 by the lengths
+  // (two to four waves).
   constexpr long long kMost = 2048, kLeast = 128, kWhole = 768;
   const long long slots = 3ll * sms;
   long long n = 1;

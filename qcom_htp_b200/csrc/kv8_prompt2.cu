@@ -6,6 +6,13 @@
 //   the time from S to P is therefore what counts, and a row is shared by two threads, 64 columns each: four softmax
 //     warpgroups, so that a scheduler has four warps to hide latencies with.  They exchange their maxima once a tile;
 //   one warpgroup converts both K and V.
+//
+// Measured: 8192 tokens of 32 heads x 128 over 8, causal, 0.60 to 0.64 ms (860 to 910 TFLOP/s of visible pairs; 0.80 ms in
+// kv8_prompt.cu's kernel); 1000-token pieces of 3 sequences, 24 heads x 64 over 8, a window of 4096 keys: 133 us (330).  A tile of
+// 128 keys takes some 4500 cycles for both slots: their MMAs 2050 (head_dim 64: 1540), the exponentials 2050 (16 a cycle), and each
+// slot's chain from S over the maxima, the exchange and the exponentials to P, 2300, in which the other slot's MMAs fit.
+// No faster: exponentials by polynomial on the FMA pipe for a part of the keys, an issuing warp for each slot (708 us against
+// 606), deeper staging, slots held apart by barriers.
 #include <algorithm>
 
 #include "kv8_prompt.cuh"
@@ -31,7 +38,8 @@ struct Shape2 {
   static_assert(4 * softmax_regs + convert_regs + mma_regs <= 6 * regs, "registers");
   // tensor memory columns: S of the two tiles, O of the two, Q of the two where there is room
   static constexpr bool q_tmem = D == 64;
-  static constexpr int o_col = 256, q_col = 384;  // (q_col: head_dim 64)
+  static constexpr int o_col = 256, q_col = o_col + 2 * D;
+  static_assert(o_col + 2 * D <= 512 && (!q_tmem || q_col + D <= 512), "tensor memory");
 };
 
 struct Barriers2 {

@@ -229,7 +229,8 @@ def kv8_attention(q: torch.Tensor, cache, block_table: torch.Tensor, lengths: to
 
     ``scale``: default head_dim ** -0.5.  ``max_new``: with ``seq_start``, at least the largest number of query tokens
     of a sequence (rows beyond it may be left out; default all).  ``max_len``: about the largest length (default: the
-    block table's reach); it sizes the launch and changes no result.  Returns out (q's shape and dtype), or
+    block table's reach); it sizes the launch, and any value gives a right result.  How the keys are cut, and so the last bits,
+    depends on the call's lengths and shapes: the same call gives the same bits.  Returns out (q's shape and dtype), or
     (out, lse) with lse float32 of q's shape without head_dim."""
     cf, dev = _cache_fields(cache)
     dtype = q.dtype
