@@ -36,7 +36,7 @@ constexpr int kKeys = 64;              // keys of a unit
 constexpr int kPanel = kKeys * 128;    // bytes of a [64 keys][64 f16] swizzled image
 
 struct Barriers {
-  uint64_t q_full, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_full[2], pv_done, drained, staged[2][4], taken[2][4];
+  uint64_t q_full, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_full[2], pv_done, o_full, drained, staged[2][4], taken[2][4];
 };
 
 struct Small {
@@ -131,6 +131,7 @@ __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const 
       }
       mbar_init(&bar.q_full, 256);
       mbar_init(&bar.pv_done, 1);
+      mbar_init(&bar.o_full, 1);
       mbar_init(&bar.drained, 1);
       fence_barrier_init();
     }
@@ -216,10 +217,9 @@ __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const 
         tc_fence_before();
         mbar_arrive(&bar.p_full[buf]);
       }
-      // the last product may be two phases ahead of what this warp has seen (S of a unit comes before P V of the one before
-      // it), and a parity tells only one: both are waited for
-      if (ok && units > 1) ok = warp_wait(&bar.pv_done, (units - 2) & 1, err, kErrTimeoutAccum);
-      if (ok) warp_wait(&bar.pv_done, (units - 1) & 1, err, kErrTimeoutAccum);
+      // a barrier of its own: pv_done may be one or two phases ahead of what this warp has seen, or at its end, and a parity
+      // does not tell them apart
+      if (ok) warp_wait(&bar.o_full, 0, err, kErrTimeoutAccum);
       tc_fence_after();
     }
     // the row's sum, and each half's columns of it
@@ -369,6 +369,7 @@ __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const 
           for (int e = 0; e < kKeys / 16; ++e)
             mma_ts(leader, tm + S::o_col, tm + buf * 64 + (e >> 1) * 32 + (e & 1) * 8, vd + e * (2048 >> 4), id_pv, i > 1 || e != 0);
           commit(leader, smem_u32(&bar.pv_done));
+          if (i == units) commit(leader, smem_u32(&bar.o_full));
           commit(leader, smem_u32(&bar.v_empty[at]));
         }
       }
