@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const 
         pin(x);
         float top = careful ? row_max<true>(k, 0, x, m) : row_max<false>(k, 0, x, m);
         s_half[buf][half][in_tile] = top;
-        named_barrier(1, 256);
+        named_barrier(2 + wq, 64);  // the two warps that share rows
         top = fmaxf(top, s_half[buf][half ^ 1][in_tile]);
         // raise m where it pays; rows of a warp move together, and its two halves alike
         if (__any_sync(0xffffffffu, top > m + kGrow || (m == -INFINITY && top != -INFINITY))) {

@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(Shape2<D>::threads, 1) kv8_prompt2_kernel(cons
             top = careful ? row_max<true>(k, 32 * c, x, top) : row_max<false>(k, 32 * c, x, top);
           }
           s_half[j & 1][slot][half][in_tile] = top;
-          named_barrier(1 + slot, 256);
+          named_barrier(3 + 4 * slot + wq, 64);  // the two warps that share rows
           top = fmaxf(top, s_half[j & 1][slot][half ^ 1][in_tile]);
           // raise m where it pays; rows of a warp move together, and its two halves alike.  S of this tile came after the
           // product of the last, so O stands still.
