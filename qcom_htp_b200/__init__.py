@@ -14,6 +14,6 @@ from .kv8 import Kv8Cache, kv8_attention, kv8_read, kv8_write
 from .matmul import (QuantMatMul, hmx_u8i4_to_u8_matmul, hmx_u8i8_to_u8_matmul, hmx_u16i4_to_u16_matmul,
                      hmx_u16i8_to_u16_matmul, hmx_u16i16_to_u16_matmul, lpbq_expand_i8, weights_from_wire)
 
-__all__ = ["Kv8Cache", "kv8_attention", "kv8_read", "kv8_write", "QhtpError", "QuantMatMul", "gdn_chunk_inverse", "gdn_inverse", "gdn_solve_u16", "gdnbm_solve", "hmx_u8i8_to_u8_matmul",
-           "hmx_u8i4_to_u8_matmul", "hmx_u16i8_to_u16_matmul", "hmx_u16i4_to_u16_matmul",
-           "hmx_u16i16_to_u16_matmul", "lpbq_expand_i8", "weights_from_wire"]
+__all__ = ["Kv8Cache", "QhtpError", "QuantMatMul", "gdn_chunk_inverse", "gdn_inverse", "gdn_solve_u16", "gdnbm_solve",
+           "hmx_u8i8_to_u8_matmul", "hmx_u8i4_to_u8_matmul", "hmx_u16i8_to_u16_matmul", "hmx_u16i4_to_u16_matmul",
+           "hmx_u16i16_to_u16_matmul", "kv8_attention", "kv8_read", "kv8_write", "lpbq_expand_i8", "weights_from_wire"]
