@@ -162,7 +162,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 3)  // as many as t
   }
 
   const int bs_log2 = a.pages.bs_log2, bs = 1 << bs_log2;
-  const long long seg_keys = static_cast<long long>(kSegBlocks - 1) << bs_log2;  // a segment may start inside a block
+  // A segment may start inside a block.  It is whole steps, except for a span's last: a step's group that is not there is
+  // not copied, and only the rows' own limits hide it, which lie at the end of the span and not at that of a segment.
+  const long long seg_keys = (static_cast<long long>(kSegBlocks - 1) << bs_log2) & ~(16ll * K16 - 1);
   bool ok = true;
   for (long long seg0 = keys.lo; seg0 < keys.hi; seg0 += seg_keys) {
     const int seg = static_cast<int>(seg0), seg_hi = static_cast<int>(min(static_cast<long long>(keys.hi), seg0 + seg_keys));
@@ -173,8 +175,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 3)  // as many as t
 
     const int groups = (seg_hi - seg + 15) >> 4, tiles = (groups + K16 - 1) / K16;
     auto block_at = [&](int gi) { return ((seg + min(gi, groups - 1) * 16) >> bs_log2) - blk0; };
-    // A lane per box: K and V, groups, panels.  A group that is not there, or that the table does not map, is not
-    // copied: its codes are whatever the ring holds, and its keys are hidden or their scales NaN.
+    // A lane per box: K and V, groups, panels.  A group that is not there (past the span's end), or that the table does not
+    // map, is not copied: its codes are whatever the ring holds, and its keys are hidden or their scales NaN.
     auto copy = [&](int tile, uint32_t at) {
       constexpr int kBoxes = 2 * K16 * Rg::panels;
       const int st = at % Rg::stages, gi = tile * K16 + (lane / 2) % K16, panel = lane / (2 * K16);
