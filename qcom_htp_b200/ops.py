@@ -188,4 +188,5 @@ def kv8_attention_op(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tens
 @kv8_attention_op.register_fake
 def _(q, cache_k, cache_v, k_scale, v_scale, block_table, lengths, scale=None, causal=True, window=0, seq_start=None,
       max_new=None, max_len=None):
-    return torch.empty_like(q), q.new_empty(q.shape[:-1], dtype=torch.float32)
+    # contiguous whatever q's order, as the op's are (empty_like alone would keep a transposed q's strides)
+    return torch.empty_like(q, memory_format=torch.contiguous_format), q.new_empty(q.shape[:-1], dtype=torch.float32)
