@@ -343,7 +343,7 @@ QhtpStatus qhtp_gdn_solve_u16(const uint16_t *A, int64_t n_chunks, int32_t C, in
  *
  * Writing to tile (block, kv head), float32 arithmetic: s_new = max|x| / 127 over the new rows x in it (0
  * below 2^-64).  If slot 0 is among them the tile starts anew with scale s = s_new, else s = max(old scale,
- * s_new) and, where s grew, the old codes become rint(code * (old / s)).  New codes are
+ * s_new), an old scale below 2^-64 counting as 0, and, where s grew, the old codes become rint(code * (old / s)).  New codes are
  * clamp(rint(x * (1 / s)), -127, 127).  A NaN or an infinity among the rows, or in the old scale, makes the
  * tile's scale NaN until it starts anew.  Each block that is written belongs to one sequence of the call,
  * and a sequence's tokens are written in order: a later write may start anywhere at or below the end, and

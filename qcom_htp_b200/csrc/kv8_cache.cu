@@ -4,8 +4,8 @@
 // that fall into it (all arithmetic float32, every operation correctly rounded):
 //
 //   s_new = max|X| / 127, 0 below 2^-64, NaN if X holds a NaN or an infinity
-//   s     = s_new where the tile's slot 0 is written (the tile starts anew), else max(s_old, s_new),
-//           NaN if either is not finite
+//   s     = s_new where the tile's slot 0 is written (the tile starts anew), else max(s_old, s_new) with an s_old
+//           below 2^-64 as 0, NaN if either is not finite
 //   new codes = clamp(rint(x * (1 / s)), -127, 127), 0 where s is 0 or NaN
 //   old codes = rint(c * (s_old / s)) where s grew
 //
@@ -96,7 +96,10 @@ __global__ void __launch_bounds__(kMaxThreads, NV <= 4 ? 6 : 3) kv8_write_kernel
   const int d = VN << a.vec_log2;
   int8_t* codes = (kv ? a.pages.v : a.pages.k) + tile * bs * d;
   float* scale_at = (kv ? a.pages.v_scale : a.pages.k_scale) + tile;
-  const float old = slot0 ? *scale_at : 0.0f;
+  // Below kScaleMin it counts as 0: new rows of that size would else be divided by a scale that they may be far above, or
+  // by one whose reciprocal is infinite.
+  float old = slot0 ? *scale_at : 0.0f;
+  if (old < kScaleMin) old = 0.0f;  // a NaN stays
 
   const int nvec = rows << a.vec_log2, cmask = (1 << a.vec_log2) - 1;
   auto load = [&](int i) {
@@ -132,7 +135,7 @@ __global__ void __launch_bounds__(kMaxThreads, NV <= 4 ? 6 : 3) kv8_write_kernel
     float f[VN];
     Vec<T>::load(r, f);
     uint32_t w[VN / 4];
-    // no |x| is above the s it was divided by, so no code is above 127
+    // s is 0, or at least the rows' own max|x| / 127: no code is above 127
 #pragma unroll
     for (int e = 0; e < VN / 4; ++e) {
       const uint32_t c = low_bytes(round_bits(__fmul_rn(f[4 * e], inv)), round_bits(__fmul_rn(f[4 * e + 1], inv)),
