@@ -266,9 +266,13 @@ def kv8_attention(q: torch.Tensor, cache, block_table: torch.Tensor, lengths: to
     handle = _on(stream, dev)
     arg = _ATTENTION.pack(*cf, *sf, lf, *rq, *ro, lse.data_ptr() if return_lse else 0, _DTYPE[dtype], heads, 1 if causal else 0,
                           window, scale, reach, 0, 0, handle)
-    need = L.lib.qhtp_kv8_attention_workspace_bytes(arg)
-    if need:
-        ws = _empty(q, (need,), torch.uint8, stream)
-        arg = arg[:-_TAIL.size] + _TAIL.pack(ws.data_ptr(), need, handle)
-    _call(L.lib.qhtp_kv8_attention, "qhtp_kv8_attention", dev, arg)
+
+    def launch(arg):  # both on the cache's device: the plan depends on its number of SMs
+        need = L.lib.qhtp_kv8_attention_workspace_bytes(arg)
+        if need:
+            ws = _empty(q, (need,), torch.uint8, stream)
+            arg = arg[:-_TAIL.size] + _TAIL.pack(ws.data_ptr(), need, handle)
+        return L.lib.qhtp_kv8_attention(arg)
+
+    _call(launch, "qhtp_kv8_attention", dev, arg)
     return (out, lse) if return_lse else out
