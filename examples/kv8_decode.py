@@ -23,7 +23,7 @@ import torch
 
 sys.path.insert(0, str(Path(__file__).resolve().parents[1]))
 
-from qcom_htp_b200 import Kv8Cache, QuantMatMul, kv8_attention, kv8_read, kv8_write  # noqa: E402
+from qcom_htp_b200 import Kv8Cache, QuantMatMul, kv8_attention, kv8_check, kv8_read, kv8_write  # noqa: E402
 
 ZERO = 32768
 STEP = 8.0 / 32768  # 16-bit codes of values in [-8, 8)
@@ -113,7 +113,7 @@ def run(batch: int = 16, hidden: int = 4096, q_heads: int = 32, kv_heads: int = 
         graph.replay()
         later.append((k.clone(), v.clone()))
     times[1].record()
-    torch.cuda.synchronize()
+    kv8_check()  # waits for the GPU, and raises if a kernel reported an error
     ms = times[0].elapsed_time(times[1]) / steps
 
     # the last step against attention over the rows that were never quantized

@@ -228,6 +228,10 @@ QhtpStatus qhtp_matmul_check(const QhtpMatmulPlan *plan, void *workspace, uint32
  * that code, exactly as it would for a GEMM whose pipeline stalled.  Asynchronous. */
 QhtpStatus qhtp_selftest_wait_timeout(int *err_word, int *warps_gave_up, uint64_t limit_cycles, void *stream);
 
+/* The same on the error word of one of the qhtp_kv8_attention kernels of the current device, so that qhtp_kv8_check
+ * reports it: kernel 0 few rows, 1 prompts in tiles of 128 rows, 2 prompts in tiles of 256. */
+QhtpStatus qhtp_selftest_kv8_timeout(uint32_t kernel, int *warps_gave_up, uint64_t limit_cycles, void *stream);
+
 /* Tensor-pipe rate probe (no counterpart in the reference): `ctas` CTAs (one per SM) each issue
  * `iters` rounds of four tcgen05.mma of M = 128, N = 256 -- kind 0: kind::i8 (u8 x s8, s32
  * accumulate, 32 bytes of K per instruction), kind 1: kind::f16 with bf16 operands (f32 accumulate,

@@ -10,10 +10,10 @@ from . import _lib  # noqa: F401  (loads libqhtp.so or raises)
 from ._lib import QhtpError
 from . import ops  # noqa: F401  (registers torch.ops.qhtp.*)
 from .gdn import gdn_chunk_inverse, gdn_inverse, gdn_solve_u16, gdnbm_solve
-from .kv8 import Kv8Cache, kv8_attention, kv8_read, kv8_write
+from .kv8 import Kv8Cache, kv8_attention, kv8_check, kv8_read, kv8_write
 from .matmul import (QuantMatMul, hmx_u8i4_to_u8_matmul, hmx_u8i8_to_u8_matmul, hmx_u16i4_to_u16_matmul,
                      hmx_u16i8_to_u16_matmul, hmx_u16i16_to_u16_matmul, lpbq_expand_i8, weights_from_wire)
 
 __all__ = ["Kv8Cache", "QhtpError", "QuantMatMul", "gdn_chunk_inverse", "gdn_inverse", "gdn_solve_u16", "gdnbm_solve",
            "hmx_u8i8_to_u8_matmul", "hmx_u8i4_to_u8_matmul", "hmx_u16i8_to_u16_matmul", "hmx_u16i4_to_u16_matmul",
-           "hmx_u16i16_to_u16_matmul", "kv8_attention", "kv8_read", "kv8_write", "lpbq_expand_i8", "weights_from_wire"]
+           "hmx_u16i16_to_u16_matmul", "kv8_attention", "kv8_check", "kv8_read", "kv8_write", "lpbq_expand_i8", "weights_from_wire"]

@@ -392,15 +392,14 @@ cudaError_t launch_kv8_prompt2(const Kv8Attn& a);
 
 // joins the chunks of a launch
 cudaError_t launch_kv8_combine(const Kv8Attn& a);
-// the current device's error words of the two (a wait that gave up leaves its code), read and cleared; synchronizes
-cudaError_t kv8_prompt_error(int* code, cudaStream_t stream);
-cudaError_t kv8_prompt2_error(int* code, cudaStream_t stream);
-cudaError_t kv8_decode_error(int* code, cudaStream_t stream);
-inline cudaError_t kv8_take_error(const void* symbol, int* code, cudaStream_t stream) {
-  void* at = nullptr;
-  cudaError_t e = cudaGetSymbolAddress(&at, symbol);
-  if (e == cudaSuccess) e = cudaMemcpyAsync(code, at, sizeof(int), cudaMemcpyDeviceToHost, stream);
-  if (e == cudaSuccess) e = cudaMemsetAsync(at, 0, sizeof(int), stream);
+// the current device's error words of the attention kernels: a wait that gave up leaves its code there
+cudaError_t kv8_decode_word(int** word);
+cudaError_t kv8_prompt_word(int** word);
+cudaError_t kv8_prompt2_word(int** word);
+// reads and clears one; synchronizes
+inline cudaError_t kv8_take_error(int* word, int* code, cudaStream_t stream) {
+  cudaError_t e = cudaMemcpyAsync(code, word, sizeof(int), cudaMemcpyDeviceToHost, stream);
+  if (e == cudaSuccess) e = cudaMemsetAsync(word, 0, sizeof(int), stream);
   if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
   return e;
 }

@@ -140,6 +140,9 @@ QhtpStatus plan_attention(const QhtpKv8Attention* run, Kv8Attn* a) {
   return QHTP_STATUS_OK;
 }
 
+// The attention kernels' error words, in the order of qhtp_selftest_kv8_timeout.
+constexpr cudaError_t (*kWords[])(int**) = {kv8_decode_word, kv8_prompt_word, kv8_prompt2_word};
+
 }  // namespace
 
 extern "C" {
@@ -186,16 +189,26 @@ QhtpStatus qhtp_kv8_attention(const QhtpKv8Attention* run) {
 
 QhtpStatus qhtp_kv8_check(int* device_code, void* stream) {
   int code = 0;
-  for (auto read : {kv8_decode_error, kv8_prompt_error, kv8_prompt2_error}) {
-    int one = 0;
-    const QhtpStatus st = status_from_cuda(read(&one, static_cast<cudaStream_t>(stream)));
-    if (st != QHTP_STATUS_OK) return st;
+  for (auto find : kWords) {
+    int *word = nullptr, one = 0;
+    cudaError_t e = find(&word);
+    if (e == cudaSuccess) e = kv8_take_error(word, &one, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return status_from_cuda(e);
     if (code == 0) code = one;
   }
   if (device_code != nullptr) *device_code = code;
   if (code == 0) return QHTP_STATUS_OK;
   set_last_message("kv8: a wait inside an attention kernel gave up");
   return QHTP_STATUS_RUNTIME_ERROR;
+}
+
+QhtpStatus qhtp_selftest_kv8_timeout(uint32_t kernel, int* warps_gave_up, uint64_t limit_cycles, void* stream) {
+  if (kernel >= sizeof(kWords) / sizeof(kWords[0])) return invalid("kv8: no such kernel");
+  if (warps_gave_up == nullptr) return invalid("kv8: null counter");
+  int* word = nullptr;
+  const cudaError_t e = kWords[kernel](&word);
+  if (e != cudaSuccess) return status_from_cuda(e);
+  return qhtp_selftest_wait_timeout(word, warps_gave_up, limit_cycles, stream);
 }
 
 }  // extern "C"

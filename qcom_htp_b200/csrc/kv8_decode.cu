@@ -695,6 +695,6 @@ cudaError_t launch_kv8_combine(const Kv8Attn& a) {
   return kv8::combine<256>(a);
 }
 
-cudaError_t kv8_decode_error(int* code, cudaStream_t stream) { return kv8_take_error(&kv8::g_error, code, stream); }
+cudaError_t kv8_decode_word(int** word) { return cudaGetSymbolAddress(reinterpret_cast<void**>(word), kv8::g_error); }
 
 }  // namespace qhtp

@@ -459,6 +459,6 @@ cudaError_t launch_kv8_prompt(const Kv8Attn& a) {
   }
 }
 
-cudaError_t kv8_prompt_error(int* code, cudaStream_t stream) { return kv8_take_error(&kv8::g_error, code, stream); }
+cudaError_t kv8_prompt_word(int** word) { return cudaGetSymbolAddress(reinterpret_cast<void**>(word), kv8::g_error); }
 
 }  // namespace qhtp

@@ -407,6 +407,6 @@ cudaError_t run2(const Kv8Attn& a) {
 
 cudaError_t launch_kv8_prompt2(const Kv8Attn& a) { return a.head_dim == 64 ? kv8::run2<64>(a) : kv8::run2<128>(a); }
 
-cudaError_t kv8_prompt2_error(int* code, cudaStream_t stream) { return kv8_take_error(&kv8::g_error2, code, stream); }
+cudaError_t kv8_prompt2_word(int** word) { return cudaGetSymbolAddress(reinterpret_cast<void**>(word), kv8::g_error2); }
 
 }  // namespace qhtp

@@ -19,6 +19,7 @@ every head starts on a multiple of 16 bytes.
 """
 from __future__ import annotations
 
+import ctypes as C
 import struct
 from typing import NamedTuple
 
@@ -276,3 +277,17 @@ def kv8_attention(q: torch.Tensor, cache, block_table: torch.Tensor, lengths: to
 
     _call(launch, "qhtp_kv8_attention", dev, arg)
     return (out, lse) if return_lse else out
+
+
+def kv8_check(device=None, stream=None) -> None:
+    """Synchronize ``stream`` (default: the current one) and raise if a kernel of kv8_attention on ``device`` (default: the
+    stream's, or the current one) has recorded a wait that gave up since the last check (qhtp_kv8_check), which leaves
+    the outputs of that call undefined.  No call does this by itself: it would wait for the GPU."""
+    if device is None:
+        device = _device() if stream is None else stream.device
+    with torch.cuda.device(device):
+        code = C.c_int(0)
+        handle = _current(_device()) if stream is None else stream.cuda_stream
+        st = L.lib.qhtp_kv8_check(C.byref(code), handle)
+    if st:
+        raise L.QhtpError(f"qhtp_kv8_check (device code {code.value})", st)
