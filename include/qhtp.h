@@ -365,7 +365,8 @@ typedef struct QhtpKv8Cache {
 /* The sequences of a call.  seq_start NULL: each has `tokens` rows, and row (b, t) lies at
  * b * batch_stride + t * token_stride.  seq_start int32 [batch + 1]: sequence b has the rows seq_start[b] to
  * seq_start[b + 1] of `total`, row i lies at i * token_stride, and `tokens` is at least the largest count (rows of a
- * sequence beyond that many may be left out).  Starts outside [0, total] or falling give no rows. */
+ * sequence beyond that many may be left out).  Starts outside [0, total] or falling give no rows; no row belongs to two
+ * sequences. */
 typedef struct QhtpKv8Seqs {
   const int32_t *block_table; /* [batch, max_blocks], rows table_stride apart */
   const int32_t *seq_start;

@@ -165,6 +165,10 @@ struct Kv8Attn {
   // chunks that the kernel sizes by the lengths, so that they are at most `fit` CTAs, of `chunk` keys at the least
   // (fit_place); fit = 0: into `chunks` of `chunk` keys, on a grid sized by max_len.
   int tile_rows, row_groups, chunk, chunks, fit;
+  // Row groups of all sequences (of one kv head) that parts have room for.  packed: sequence b's are behind those that the
+  // rows before it can fill (groups_before), else each sequence has room for row_groups.
+  long long part_groups;
+  int packed, tile_log2;  // tile_rows = 1 << tile_log2
   float* part;            // workspace: unnormalised rows, then their maxima and sums, then (fit) the sequences' cuts
   cudaStream_t stream;
 };
@@ -198,13 +202,25 @@ __device__ __forceinline__ Span chunk_span(const Place& p, const Span& s) {
   const long long hi = p.chunk == p.chunks - 1 ? s.hi : min(static_cast<long long>(s.hi), lo + p.keys);
   return lo < hi ? Span{static_cast<int>(lo), static_cast<int>(hi)} : Span{0, 0};
 }
+// Where the sequences' parts lie.  Of packed rows, sequence b's first row is row0 of all: the ones before it fill at most
+// floor(row0 group / tile_rows) row groups and begin at most b more, one for each sequence.
+__host__ __device__ __forceinline__ long long groups_before(const Kv8Attn& a, long long b, long long row0) {
+  return a.packed ? ((row0 * a.group) >> a.tile_log2) + b : b * a.row_groups;
+}
+__host__ inline void place_parts(Kv8Attn& a) {
+  const long long all = static_cast<long long>(a.seqs.batch) * a.row_groups;
+  a.tile_log2 = 0;
+  while ((1 << a.tile_log2) < a.tile_rows) ++a.tile_log2;
+  a.packed = 1;
+  a.part_groups = groups_before(a, a.seqs.batch, a.seqs.total);
+  if (a.seqs.start == nullptr || a.part_groups >= all) a.packed = 0, a.part_groups = all;
+}
 // Offset of a (sequence, kv head, row group, chunk) part in rows.
-__device__ __forceinline__ long long part_row(const Kv8Attn& a, int b, int h, int rg, int c) {
-  return (((static_cast<long long>(b) * a.pages.heads + h) * a.row_groups + rg) * a.chunks + c) * a.tile_rows;
+__device__ __forceinline__ long long part_row(const Kv8Attn& a, int b, long long row0, int h, int rg, int c) {
+  return (((groups_before(a, b, row0) + rg) * a.pages.heads + h) * a.chunks + c) * a.tile_rows;
 }
 __host__ __device__ __forceinline__ long long part_rows(const Kv8Attn& a) {
-  if (a.fit) return static_cast<long long>(a.fit) * a.tile_rows;
-  return static_cast<long long>(a.seqs.batch) * a.pages.heads * a.row_groups * a.chunks * a.tile_rows;
+  return (a.fit ? a.fit : a.part_groups * a.pages.heads * a.chunks) * a.tile_rows;
 }
 
 // Cutting the keys by the lengths.  A grid sized on the host has to be sized for the longest sequence that there may be:

@@ -58,8 +58,9 @@ kv8::Pages pages_of(const QhtpKv8Cache& c) {
   return {c.k, c.v, c.k_scale, c.v_scale, c.num_blocks, static_cast<int>(c.kv_heads), log2};
 }
 kv8::Seqs seqs_of(const QhtpKv8Seqs& s) {
+  // no start reaches past 2^31 - 1, and products of total stay in 64 bits
   return {s.block_table,  s.table_stride, static_cast<int>(s.max_blocks), static_cast<int>(s.batch), s.seq_start,
-          static_cast<int>(s.tokens), s.total};
+          static_cast<int>(s.tokens), s.total < 0x7fffffff ? s.total : 0x7fffffff};
 }
 kv8::Rows rows_of(const QhtpKv8Rows& r) { return {r.data, r.batch_stride, r.token_stride, r.head_stride}; }
 
@@ -134,6 +135,7 @@ QhtpStatus plan_attention(const QhtpKv8Attention* run, Kv8Attn* a) {
     kv8_prompt_plan(*a, sm_count());
   else
     kv8_decode_plan(*a, sm_count());
+  kv8::place_parts(*a);
   if (a->prompt && a->row_groups > 65535) return unsupported("kv8: too many rows");
   if (static_cast<long long>(a->chunks) * a->pages.heads > (1ll << 30)) return unsupported("kv8: too many chunks");
   if (static_cast<long long>(a->pages.heads) * a->row_groups > (1ll << 30)) return unsupported("kv8: too many rows");

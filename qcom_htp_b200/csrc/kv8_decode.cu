@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 3)  // as many as t
   } else {
     // chunks slowest: the first ones, which every sequence has whole, run first, and the remainders fill the end
     at.b = blockIdx.y, at.h = blockIdx.x / a.row_groups, at.rg = blockIdx.x - at.h * a.row_groups, at.chunk = blockIdx.z;
-    at.chunks = a.chunks, at.keys = a.chunk, at.part = part_row(a, at.b, at.h, at.rg, at.chunk);
+    at.chunks = a.chunks, at.keys = a.chunk;
   }
   const int b = at.b, h = at.h;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 3)  // as many as t
     __syncthreads();
   }
 
-  const long long part = s_place.part;
+  const long long part = FIT ? s_place.part : part_row(a, b, row0, h, s_place.rg, s_place.chunk);
   const bool whole = s_place.chunks == 1;
   for (int i = threadIdx.x; i < kRows * (D / 8); i += kWarps * 32) {
     const int r = i / (D / 8), c = i - r * (D / 8), row = r0 + r;
@@ -476,7 +476,7 @@ __device__ __forceinline__ Parts parts_of(const Kv8Attn& a, int row) {
     p.first = static_cast<long long>(cut.x + cut.w - (rg + 1) * a.pages.heads + p.h) * a.tile_rows;
     p.step = static_cast<long long>(cut.w) * a.tile_rows;
   } else {
-    p.first = part_row(a, p.b, p.h, rg, 0);
+    p.first = part_row(a, p.b, p.row0, p.h, rg, 0);
     p.step = a.tile_rows;
   }
   p.first += row - r0;

@@ -94,11 +94,12 @@ __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const 
     // heads fastest, the longest row groups (the last of a causal sequence) first
     place.h = blockIdx.x / a.chunks, place.chunk = blockIdx.x - place.h * a.chunks, place.b = blockIdx.y;
     place.rg = a.row_groups - 1 - blockIdx.z;
-    place.chunks = a.chunks, place.keys = a.chunk, place.part = part_row(a, place.b, place.h, place.rg, place.chunk);
+    place.chunks = a.chunks, place.keys = a.chunk;
   }
   const int b = place.b, h = place.h;
   long long row0;
   const int T = seq_rows(a.seqs, b, row0);
+  if constexpr (!FIT) place.part = part_row(a, b, row0, h, place.rg, place.chunk);
   const int R = T * a.group, r0 = place.rg * 128;
   if (r0 >= R) return;
   const int r1 = min(R, r0 + 128);
