@@ -420,7 +420,9 @@ typedef struct QhtpKv8Attention {
   void *stream;
 } QhtpKv8Attention;
 
-/* Device workspace of the call (0 for many): reads the shapes, dtype, window and max_len of *run only. */
+/* Device workspace of the call on the current device: 0 for many, and for a call that would be refused.  Looks at every
+ * number in *run and at whether seq_start is NULL, so fill those in first; the other pointers are not looked at, and none is
+ * followed. */
 size_t qhtp_kv8_attention_workspace_bytes(const QhtpKv8Attention *run);
 QhtpStatus qhtp_kv8_attention(const QhtpKv8Attention *run);
 

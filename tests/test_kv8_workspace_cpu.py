@@ -40,3 +40,25 @@ def test_a_total_that_no_start_can_reach(total):
     c = (8, total, 32, 8, 128, 700)
     need = L.lib.qhtp_kv8_attention_workspace_bytes(C.byref(call(*c)))
     assert need <= 8 * 8 * (700 * 4 // 256 + 1) * 2 * 256 * 130 * 4  # two chunks of every sequence's row groups
+
+
+def test_the_size_looks_at_numbers_and_seq_start_only():
+    """No pointer but seq_start matters to the size; seq_start does (packed rows are cut by their total), and so does whether the call
+    would be refused."""
+    def size(**kw):
+        run = call(8, 1400, 32, 8, 128, 1400)
+        for name, value in kw.items():
+            *path, last = name.split("__")
+            at = run
+            for p in path:
+                at = getattr(at, p)
+            setattr(at, last, value)
+        return L.lib.qhtp_kv8_attention_workspace_bytes(C.byref(run))
+
+    full = size()
+    assert full > 0
+    for name in ("cache__k", "cache__v", "cache__k_scale", "cache__v_scale", "seqs__block_table", "lengths", "q__data", "out__data", "stream"):
+        assert size(**{name: None}) == full
+    assert size(seqs__seq_start=None) != full
+    for bad in (dict(scale=0.0), dict(dtype=2), dict(q_heads=31), dict(causal=0, window=5)):
+        assert size(**bad) == 0
