@@ -316,9 +316,9 @@ __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const 
                     &bar.staged[v][st]);
         }
       }
-      if (i < units)  // a wait gave up: copies under way end before the block does
-        for (int n = max(0, i - S::depth); n < i; ++n)
-          warp_wait(&bar.staged[v][n % S::depth], (n / S::depth) & 1, err, kErrTimeoutOther);
+      // copies under way end before the block does, also where a wait gave up, here or in the converters that take them
+      for (int n = max(0, i - S::depth); n < i; ++n)
+        warp_wait(&bar.staged[v][n % S::depth], (n / S::depth) & 1, err, kErrTimeoutOther);
     } else if (warp == kScale) {
       // ----------------------------------------------------------------------------- scales
       int id_next = ids_of(1);
@@ -374,10 +374,10 @@ __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const 
           commit(leader, smem_u32(&bar.v_empty[at]));
         }
       }
-      if (!ok) {  // a wait gave up: nothing issued here may run on when tensor memory is freed
-        commit(leader, smem_u32(&bar.drained));
-        warp_wait(&bar.drained, 0, err, kErrTimeoutOther);
-      }
+      // nothing issued here may run on when tensor memory is freed: where a wait gave up, here or in the softmax warps, no one
+      // else has waited for it
+      commit(leader, smem_u32(&bar.drained));
+      warp_wait(&bar.drained, 0, err, kErrTimeoutOther);
     }
   }
   tc_fence_before();

@@ -300,9 +300,9 @@ __global__ void __launch_bounds__(Shape2<D>::threads, 1) kv8_prompt2_kernel(cons
                     16 * D, &bar.staged[at]);
         }
       }
-      if (!ok)  // copies under way end before the block does
-        for (int i = max(0, n - kStaged); i < n; ++i)
-          warp_wait(&bar.staged[i % kStaged], (i / kStaged) & 1, err, kErrTimeoutOther);
+      // copies under way end before the block does, also where a wait gave up, here or in the converters that take them
+      for (int i = max(0, n - kStaged); i < n; ++i)
+        warp_wait(&bar.staged[i % kStaged], (i / kStaged) & 1, err, kErrTimeoutOther);
     } else if (warp == kScale) {
       int id_next = ids_of(1);
       RawScales sc = tiles > 0 ? raw_scales(a, ids_of(0), h) : RawScales{};
@@ -364,10 +364,10 @@ __global__ void __launch_bounds__(Shape2<D>::threads, 1) kv8_prompt2_kernel(cons
           }
         }
       }
-      if (!ok) {  // a wait gave up: nothing issued here may run on when tensor memory is freed
-        commit(leader, smem_u32(&bar.drained));
-        warp_wait(&bar.drained, 0, err, kErrTimeoutOther);
-      }
+      // nothing issued here may run on when tensor memory is freed: where a wait gave up, here or in the softmax warps, no one
+      // else has waited for it
+      commit(leader, smem_u32(&bar.drained));
+      warp_wait(&bar.drained, 0, err, kErrTimeoutOther);
     }
   }
   tc_fence_before();
