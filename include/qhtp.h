@@ -403,7 +403,8 @@ QhtpStatus qhtp_kv8_read(const QhtpKv8Move *move);
  * position p = lengths[b] - T + t, and with `causal` sees the keys 0..p, with `window` > 0 (causal only) the
  * keys p - window + 1..p, else all of them.  A row that sees no key gives zeros.  A negative length counts as 0, one
  * past the block table as its end.  Scores, maxima, sums and outputs are float32; q is taken to f16 by a power
- * of two per row (all bits of elements within 2^-29 of the row's largest), probabilities are rounded to f16.
+ * of two per row (all bits of elements within 2^-29 of the row's largest), probabilities (times their V scales) are rounded
+ * to f16, each within 2^-11 of itself or 2^-32 of the row's largest; below 2^-133 of that they count as 0, also in the sum.
  * Scales are at least 0; a V scale below 2^-64 counts as 0. */
 typedef struct QhtpKv8Attention {
   QhtpKv8Cache cache;

@@ -338,6 +338,12 @@ __device__ __forceinline__ bool fit_place(const Kv8Attn& a, int cta, int2* memor
   return there;
 }
 
+// Exponents are taken to m - kLift, so that a row's p are 2^7 where t = m.  As f16 operands they keep 11 bits down to 2^-14,
+// 2^-21 of that, and below it are off by 2^-25, 2^-32 of it: 2^20 keys of small p, which may be all of the output where the
+// largest p's key has a small value, then lose no more than f16's 11 bits do.  (At kLift 0 thousands of keys of 2^-25 each were
+// off by a quarter.)  The prompt kernels let p pass that by 2^8 (kGrow): 2^15, inside f16.
+constexpr float kLift = 7.0f;
+
 // mbar_wait for a whole warp: every lane goes on, or none does.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int code) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));

@@ -1,11 +1,11 @@
 // Attention of few query rows (single tokens, drafted tokens) over the 8-bit paged KV cache.
 //
-// Per row:  t_j = q . ck_j * (scale log2(e) sk) + log2(sv),   p_j = 2^(t_j - m),   m the running maximum of t
+// Per row:  t_j = q . ck_j * (scale log2(e) sk) + log2(sv),   p_j = 2^(t_j - m),   m the running maximum of t less kLift
 //           out = sum_j p_j cv_j / sum_j p_j / sv,            lse = ln 2 (m + log2(sum_j p_j / sv))
 // with ck, cv the int8 codes of key j and sk, sv the scales of its block.  V's scale enters the
 // exponent, so the codes themselves are the tensor core's operands (int8 is exact in f16), a scale
-// costs nothing per element, and since the maximum is taken over t the largest p is 1: p rounded to f16
-// loses at most 2^-12 of what it adds to the output.  Scores, maxima, sums and outputs are float32.
+// costs nothing per element, and since the maximum is taken over t the largest p is 2^kLift: p rounded to f16 is off by at
+// most 2^-11 of itself, and a small one by 2^-32 of the largest.  Scores, maxima, sums and outputs are float32.
 //
 // Bound by memory: two bytes per key and element.  The keys of a (sequence, kv head) are cut into chunks
 // over the grid, a CTA's four warps take 32 of them (16 at head_dim 256) in turn, and each warp keeps a ring of
@@ -311,11 +311,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 3)  // as many as t
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) top[n][i] = fmaxf(top[n][i], __shfl_xor_sync(0xffffffffu, top[n][i], x));
-          // a row that has seen nothing yet keeps the maximum -inf; its terms are 2^-inf against 0
+          // a row that has seen nothing yet keeps the maximum -inf; its terms are 2^-inf against 0 (less kLift)
           const float base = top[n][i] == -INFINITY ? 0.0f : top[n][i];
           const float alpha = ex2(m[n][i] - base);
           m[n][i] = top[n][i];
-          top[n][i] = base;
+          top[n][i] = base - kLift;
           l[n][i] *= alpha;
 #pragma unroll
           for (int t = 0; t < MT; ++t) acc[n][t][i] *= alpha, acc[n][t][i + 2] *= alpha;
@@ -444,14 +444,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 3)  // as many as t
       for (int w = 0; w < kAreas; ++w) o[e] += s_o[w * kArea + r * kOStride + 8 * c + e];
     }
     if (whole) {
-      write_row8(a, b, row0, row, h, 8 * c, o, sum, base);
+      write_row8(a, b, row0, row, h, 8 * c, o, sum, base - kLift);
     } else {
       float4* to = reinterpret_cast<float4*>(a.part + (part + r) * D + 8 * c);
       to[0] = make_float4(o[0], o[1], o[2], o[3]);
       to[1] = make_float4(o[4], o[5], o[6], o[7]);
       if (c == 0) {
         float* ml = a.part + part_rows(a) * D + 2 * (part + r);
-        ml[0] = base, ml[1] = sum;
+        ml[0] = base - kLift, ml[1] = sum;
       }
     }
   }

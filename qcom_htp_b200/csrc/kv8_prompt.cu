@@ -14,8 +14,8 @@
 // There are two S buffers, so that the softmax of one unit runs under the MMAs of its neighbours.  Q stands in tensor
 // memory: an MMA of 64 columns then reads 2 KB of shared memory where it would read 6.
 //
-// m is raised, and O rescaled, only when a row's maximum has grown by more than 2^8: p then stays below
-// 2^8, far inside f16, and most units leave O alone.
+// m is raised, and O rescaled, only when a row's maximum has grown by more than 2^8: p, taken to m - kLift, then stays below
+// 2^15, inside f16, and most units leave O alone.
 //
 // Measured: 2 prompts of up to 2500 tokens, 16 heads x 256 over 2: 93 us (640 TFLOP/s of visible pairs); 6 tokens of 28 heads x 128
 // over 4 of each of 16 sequences of up to 4100 keys: 28 us.  A unit of 64 keys takes some 1600 cycles (head_dim 128) to 2500 (256):
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const 
           l *= alpha;
           m = top;
         }
-        const float base = m == -INFINITY ? 0.0f : m;
+        const float base = (m == -INFINITY ? 0.0f : m) - kLift;
         l = careful ? row_exp<true>(k, 0, x, base, l, w) : row_exp<false>(k, 0, x, base, l, w);
         tmem_st16(s_at, w);
         tmem_st_wait();
@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(Shape<D>::threads, 1) kv8_prompt_kernel(const 
     s_half[units & 1][half][in_tile] = l;
     named_barrier(1, 256);
     l = s_half[units & 1][0][in_tile] + s_half[units & 1][1][in_tile];
-    const float base = m == -INFINITY ? 0.0f : m;
+    const float base = (m == -INFINITY ? 0.0f : m) - kLift;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const long long part0 = small.place.part + wq * 32, part = part0 + lane;
     // K's images are free: every S has been computed.  Rows of head_dim 64 are one piece, which the first half's warp takes.

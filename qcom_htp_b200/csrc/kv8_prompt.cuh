@@ -7,7 +7,8 @@ namespace kv8 {
 namespace {
 
 constexpr int kQPanel = 128 * 128;     // bytes of a [128 rows][64 f16] image of Q
-constexpr float kGrow = 8.0f;          // log2 of how far p may pass 1 before m follows
+constexpr float kGrow = 8.0f;          // log2 of how far p may pass 2^kLift before m follows
+static_assert(kGrow + kLift <= 15.0f, "p and its rounding stay inside f16");
 
 template <int N>
 __device__ __forceinline__ void reg_alloc() {

@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(Shape2<D>::threads, 1) kv8_prompt2_kernel(cons
             l *= alpha;
             m = top;
           }
-          const float base = m == -INFINITY ? 0.0f : m;
+          const float base = (m == -INFINITY ? 0.0f : m) - kLift;
           // p of 32 keys over the first half of their own columns of S; the last ones are still in x
 #pragma unroll
           for (int c = 1; c >= 0; --c) {
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(Shape2<D>::threads, 1) kv8_prompt2_kernel(cons
       s_half[tiles & 1][slot][half][in_tile] = l;
       named_barrier(1 + slot, 256);
       l = s_half[tiles & 1][slot][0][in_tile] + s_half[tiles & 1][slot][1][in_tile];
-      const float base = m == -INFINITY ? 0.0f : m;
+      const float base = (m == -INFINITY ? 0.0f : m) - kLift;
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       const int rw = sr0 + wq * 32;
       const long long part0 = s_place.part + slot * 128 + wq * 32, part = part0 + lane;
