@@ -103,8 +103,12 @@ def _rows_fields(name, t, heads, head_dim, dtype, dev, ragged):
         bs, ts, hs = 0, s[0], s[1]
     else:
         bs, ts, hs, _ = s
-    if (ptr | (bs | ts | hs) * (4 if dtype is torch.float32 else 2)) & 15:
-        raise ValueError(f"{name}: every head must start on a multiple of 16 bytes")
+    size = 4 if dtype is torch.float32 else 2
+    if (ptr | (bs | ts | hs) * size) & 15:
+        # the stride of an axis of extent 1 moves nothing, and may be anything
+        bs, ts, hs = (stride if n > 1 else 0 for stride, n in zip((bs, ts, hs), shape if not ragged else (1, *shape)))
+        if (ptr | (bs | ts | hs) * size) & 15:
+            raise ValueError(f"{name}: every head must start on a multiple of 16 bytes")
     return ptr, bs, ts, hs
 
 
