@@ -414,7 +414,7 @@ typedef struct QhtpKv8Attention {
   float *lse;                 /* [rows, q_heads] natural log of the sums of exponentials, -inf for no key; may be NULL */
   uint32_t dtype, q_heads;
   uint32_t causal, window;
-  float scale;                /* finite, > 0 */
+  float scale;                /* > 0, and finite times log2(e) */
   uint32_t max_len;           /* about the largest length: sizes the launch; any value gives a right result */
   void *workspace;            /* qhtp_kv8_attention_workspace_bytes; 256-byte aligned */
   size_t workspace_bytes;

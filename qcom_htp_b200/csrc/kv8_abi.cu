@@ -119,6 +119,7 @@ QhtpStatus plan_attention(const QhtpKv8Attention* run, Kv8Attn* a) {
   a->causal = run->causal != 0;
   a->window = static_cast<int>(run->window);
   a->scale_log2 = run->scale * 1.44269504088896341f;
+  if (!std::isfinite(a->scale_log2)) return invalid("kv8: scale times log2(e) must be finite");
   a->bf16 = run->dtype == QHTP_DTYPE_BF16;
   const long long cap = static_cast<long long>(run->seqs.max_blocks) * run->cache.block_size;
   a->max_len = static_cast<int>(run->max_len < cap ? run->max_len : cap);

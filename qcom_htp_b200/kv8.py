@@ -30,6 +30,7 @@ from . import _lib as L
 HEAD_DIMS = (64, 128, 256)
 BLOCK_SIZES = (16, 32, 64, 128)
 _DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_SCALE_MOST = 2.35e38  # times log2(e) still a float32
 # QhtpKv8Move and QhtpKv8Attention, packed in one call (native sizes and alignment)
 _MOVE = struct.Struct("@4Pq4I 2P2q4I P P3q P3q 2I P")
 _ATTENTION = struct.Struct("@4Pq4I 2P2q4I P P3q P3q P 4I f I P N P")
@@ -255,8 +256,8 @@ def kv8_attention(q: torch.Tensor, cache, block_table: torch.Tensor, lengths: to
         raise ValueError("window must be 0, or positive and causal")
     if scale is None:
         scale = d ** -0.5
-    if not 0.0 < scale < float("inf"):
-        raise ValueError("scale must be finite and above 0")
+    if not 2.0 ** -149 <= scale <= _SCALE_MOST:
+        raise ValueError("scale must be above 0 and no more than 2.35e38, in float32")
     if out is None:  # contiguous
         out, ts = _like(q, stream), heads * d
         ro = out.data_ptr(), 0 if ragged else tokens * ts, ts, d
