@@ -62,6 +62,8 @@ def _cache_fields(cache):
     shape = k.shape
     if len(shape) != 4 or v.shape != shape or ks.shape != shape[:2] or vs.shape != ks.shape:
         raise ValueError("the cache is int8 [num_blocks, kv_heads, block_size, head_dim] twice and float32 [num_blocks, kv_heads] twice")
+    if 0 in shape:
+        raise ValueError("the cache needs blocks and heads")
     if not (k.dtype is v.dtype is torch.int8 and ks.dtype is vs.dtype is torch.float32):
         raise TypeError("the cache's codes must be int8 and its scales float32")
     if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
@@ -119,6 +121,8 @@ def _counts(t, seq_start, most, what):
         if t.dim() != 4:
             raise ValueError(f"{what} must be [batch, tokens, heads, head_dim], or come with seq_start")
         return t.shape[1], 0
+    if t.dim() != 3:
+        raise ValueError(f"{what} must be [rows, heads, head_dim] with seq_start")
     total = t.shape[0]
     return total if most is None else max(0, min(int(most), total)), total
 
@@ -207,12 +211,14 @@ def kv8_read(cache, block_table: torch.Tensor, first: torch.Tensor, tokens: int 
         if total is None or tokens is not None or total < 0:
             raise ValueError("a read with seq_start takes total (the rows in all) instead of tokens")
         shape = (total, heads, d)
-        tokens = total if max_tokens is None else min(int(max_tokens), total)
+        tokens = total if max_tokens is None else max(0, min(int(max_tokens), total))
     else:
         if tokens is None or tokens < 0:
             raise ValueError("tokens must be given, or seq_start and total")
-        shape, total = (block_table.shape[0], tokens, heads, d), 0
+        total = 0
     sf = _seqs_fields(block_table, seq_start, tokens, total, dev)
+    if not ragged:
+        shape = (sf[5], tokens, heads, d)
     pf = _ints("first", first, sf[5], dev)
     k = _empty(first, shape, dtype, stream)
     v = _like(k, stream)
@@ -252,8 +258,8 @@ def kv8_attention(q: torch.Tensor, cache, block_table: torch.Tensor, lengths: to
         raise ValueError("q's heads must be a multiple of the cache's")
     rq = _rows_fields("q", q, heads, d, dtype, dev, ragged)
     lf = _ints("lengths", lengths, b, dev)
-    if window < 0 or (window and not causal):
-        raise ValueError("window must be 0, or positive and causal")
+    if not 0 <= window <= 1 << 30 or (window and not causal):
+        raise ValueError("window must be 0, or positive (up to 2^30) and causal")
     if scale is None:
         scale = d ** -0.5
     if not 2.0 ** -149 <= scale <= _SCALE_MOST:
