@@ -130,7 +130,7 @@ QhtpStatus plan_attention(const QhtpKv8Attention* run, Kv8Attn* a) {
   }
   // Rows of a (sequence, kv head) that one group of the few-row kernel holds stay there; more would read the keys once per group.
   // Measured: 24 rows of head_dim 64 41 us there, 53 on the prompt kernels; 42 rows of head_dim 128 54 and 37, 48 rows 163 and 63;
-  // 40 rows of head_dim 256 54 and 32.
+  // 40 rows of head_dim 256 54 and 32.  (Above 16 rows with keys cut for three CTAs an SM where two fit.)
   a->prompt = static_cast<long long>(a->seqs.tokens) * a->group > (a->head_dim == 256 ? 16 : 32);
   if (a->prompt)
     kv8_prompt_plan(*a, sm_count());

@@ -12,14 +12,15 @@
 // One CTA owns one tile of K or of V, so a tile's scale, its old codes and its new ones are read and
 // written by that CTA alone: no atomics, and the same bytes in every run.
 //
-// Bound by memory: per element the input is read once (2 or 4 bytes) and one code byte is written; a
+// Per element the input is read once (2 or 4 bytes) and one code byte is written; a
 // tile's rows stay in registers between the maximum and the rounding.  Conversions between integers and floats run at a
 // quarter of the rate of additions and took longer than the memory here, so both directions go through additions:
 // y + 1.5 2^23 leaves rint(y) in its low bits, and 2^23 + (code + 128) is made by placing a byte (20446 tokens of 8 heads
 // x 128 written and read back: 93 us with conversions, 76 without).
 //
-// Measured, 8 heads x 128, blocks of 64: 20446 f16 tokens of 8 sequences written in 29 us (4.3 TB/s), read as f32 in 41 us
-// (5.1 TB/s); 80000 tokens read as bf16 in 83 us (5.9 TB/s).  One token of each of 64 sequences is written in 4.5 us, which is the
+// Measured, 8 heads x 128, blocks of 64: 20446 f16 tokens of 8 sequences written in 29 us (4.3 TB/s; 20480 in 8 equal ones 27, of
+// f32 44 us, 4.7 TB/s), read as f32 in 41 us (5.1 TB/s); 80000 tokens read as bf16 in 83 us (5.9 TB/s).  A write keeps neither
+// memory nor issue slots (66 %) busy throughout: each small CTA loads, waits, and stores.  One token of each of 64 sequences is written in 4.5 us, which is the
 // chain of a CTA's loads (position, table, old scale and row, old codes where the scale grew), not their bytes.
 // Persistent CTAs that fetch the next tile's rows ahead were slower (107 us against 93): the many small CTAs that an SM holds
 // overlap better.

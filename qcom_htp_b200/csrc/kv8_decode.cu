@@ -10,7 +10,8 @@
 // Bound by memory: two bytes per key and element.  The keys of a (sequence, kv head) are cut into chunks
 // over the grid, a CTA's four warps take 32 of them (16 at head_dim 256) in turn, and each warp keeps a ring of
 // them in shared memory filled by TMA, so that the loads in flight do not hang on registers or on what the warp does.
-// Measured: 2 sequences of 131072 keys, 8 kv heads x 128, 90 us (6.0 TB/s; 6.4 to 6.5 between the first loads and the last);
+// Measured: 2 sequences of 131072 keys, 8 kv heads x 128, 90 us (6.0 TB/s; 6.4 to 6.5 between the first loads and the last; the
+// same with blocks of 16, 32, 64 and 128);
 // 64 of 4000 on average 101 us (5.3 TB/s); 16 of 9500 on average, 2 x 256, 35 us (4.4 TB/s).  What is left is a CTA's start
 // (some 4 us until its first keys arrive) and the last CTAs' end, and the join (3 to 5 us).
 // Keys are the M side of the MMAs (m16n8k16, S^T = K Q^T and O^T = V^T P^T), so a group of eight query rows
@@ -73,7 +74,7 @@ struct Ring {
 
 // FIT: cut by fit_place, else on the plan's grid.  Two kernels, since that code costs the other one registers.
 template <int D, int NT, bool FIT>
-__global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 3)  // as many as the rings leave room for
+__global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 3)  // what the rings leave room for; of <256, 2> two
     kv8_decode_kernel(const Kv8Attn a, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
   using Rg = Ring<D, NT>;
   constexpr int K16 = Rg::k16;
@@ -647,7 +648,8 @@ void kv8_decode_plan(Kv8Attn& a, int sms) {
   long long span = a.max_len;
   if (a.window) span = std::min(span, static_cast<long long>(a.window) + a.tile_rows + 31);
   span = std::max(span, 1ll);
-  // Three CTAs fit an SM.  Where the row groups alone are many waves of those, chunks of kMost keys are short enough for
+  // Three CTAs fit an SM up to 16 rows, two with 32 (registers) and with 16 rows of head_dim 256 (shared memory), for which
+  // the rules below, made for three, cut the keys into one and a half waves.  Where the row groups alone are many waves of those, chunks of kMost keys are short enough for
   // sequences of unlike lengths to share the SMs.  Else the keys are cut so that the CTAs are one whole wave (by the lengths:
   // fit_place).  Short spans are left whole: a CTA takes 512 keys in less time than a second kernel needs to join two parts.
   // Measured, 2 x 131072 keys: one wave 95.6 us, two 103.2, three 109.3, chunks of 2048 keys (2.3 waves) 110.

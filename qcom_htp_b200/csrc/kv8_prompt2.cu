@@ -7,7 +7,7 @@
 //     warpgroups, so that a scheduler has four warps to hide latencies with.  They exchange their maxima once a tile;
 //   one warpgroup converts both K and V.
 //
-// Measured: 8192 tokens of 32 heads x 128 over 8, causal, 0.60 to 0.64 ms (860 to 910 TFLOP/s of visible pairs; 0.80 ms in
+// Measured: 8192 tokens of 32 heads x 128 over 8, causal, 0.60 to 0.65 ms (850 to 910 TFLOP/s of visible pairs; 0.80 ms in
 // kv8_prompt.cu's kernel); 1000-token pieces of 3 sequences, 24 heads x 64 over 8, a window of 4096 keys: 133 us (330).  A tile of
 // 128 keys takes some 4500 cycles for both slots: their MMAs 2050 (head_dim 64: 1540), the exponentials 2050 (16 a cycle), and each
 // slot's chain from S over the maxima, the exchange and the exponentials to P, 2300, in which the other slot's MMAs fit.
